@@ -248,6 +248,7 @@ _lib: Optional[C.CDLL] = None
 _VP = C.c_void_p
 _FP = C.c_void_p  # float pointers are passed as raw addresses (host or device)
 _I = C.c_int
+_LL = C.c_longlong
 
 
 def _declare(lib: C.CDLL) -> None:
@@ -348,6 +349,17 @@ def _declare(lib: C.CDLL) -> None:
         "ab200_mvm_forward_noalloc": (
             _I, [C.POINTER(IOParams), _FP, _I, _I, _FP, _FP, _I, C.c_uint64, C.c_uint32, _VP]
         ),
+        "ab200_dropout": (_I, [_VP, _LL, _VP, _LL, _VP, _LL, _LL, _I, _I, C.c_double, C.c_uint64, C.c_uint32, _VP]),
+        "ab200_layer_norm_forward": (_I, [_VP, _LL, _VP, _LL, _VP, _VP, _VP, _LL, _VP, _LL, _VP, _VP, _LL, _I, _I, _I,
+                                          C.c_float, C.c_double, C.c_uint64, C.c_uint32, _VP]),
+        "ab200_layer_norm_workspace": (_I, [_LL, _I, C.POINTER(_LL)]),
+        "ab200_layer_norm_backward": (_I, [_VP, _LL, _VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _VP, _VP, _LL, _VP, _LL, _VP, _VP,
+                                           _VP, _LL, _I, _I, _I, C.c_double, C.c_uint64, C.c_uint32, _VP]),
+        "ab200_low_rank_apply": (_I, [_VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _VP, _VP, _VP, _I, _LL, _I, _I, _I, _I,
+                                      _I, _VP, _VP]),
+        "ab200_low_rank_grad_workspace": (_I, [_LL, _I, _I, _I, _I, _I, C.POINTER(_LL)]),
+        "ab200_low_rank_grad": (_I, [_VP, _LL, _VP, _VP, _I, _VP, _LL, _VP, _VP, _I, _VP, _VP, _I, _LL, _I, _I, _I,
+                                     _VP, _VP]),
         "ab200_set_mvm_path": (_I, [_I]),
         "ab200_set_update_path": (_I, [_I]),
         "ab200_measure_popc_peak": (_I, [_I, C.POINTER(C.c_double)]),

@@ -19,6 +19,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(CSRC, "libaihwkit_b200.so")
 OBJ = os.path.join(CSRC, "build")
+DIGITAL_OUT = os.path.join(CSRC, "ab200_digital.so")  # torch binding of the digital operators
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -75,6 +76,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    _build_digital(force)
     if verbose:
         for src, log in logs.items():
             print(f"== {os.path.basename(src)}\n{log}")
@@ -82,6 +84,29 @@ def build(force: bool = False, verbose: bool = False) -> str:
         for src, log in logs.items():
             f.write(f"== {os.path.basename(src)}\n{log}\n")
     return OUT
+
+
+def _build_digital(force: bool) -> None:
+    """Compile ``csrc/digital_module.cpp``, the torch binding of ``aihwkit_b200.digital`` over the C ABI."""
+    src = os.path.join(CSRC, "digital_module.cpp")
+    include = os.path.join(os.path.dirname(HERE), "include")
+    if not force and not _stale(DIGITAL_OUT, [src, os.path.join(include, "aihwkit_b200.h")]):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.isabs(_nvcc()) else "/usr/local/cuda"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=ab200_digital",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", DIGITAL_OUT, f"-I{include}",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{os.path.join(cuda, 'include')}"]
+    cmd += [f"-I{d}" for d in include_paths()] + [f"-L{d}" for d in library_paths()]
+    cmd += [f"-L{CSRC}", "-laihwkit_b200", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+            "-ltorch_cuda", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{res.stdout}\n{res.stderr}")
 
 
 def build_pybind(verbose: bool = False):

@@ -2,6 +2,7 @@
 // exceptions into return codes + ab200_last_error(), like the reference's binding turns
 // std::runtime_error into Python RuntimeError.
 #include "array.h"
+#include "digital.h"
 #include "tile.h"
 
 #include <algorithm>
@@ -1051,6 +1052,176 @@ int ab200_set_update_path(int mode) {
     AB200_FATAL("set_update_path: mode must be 0, 1 or 2");
   }
   ab200::setUpdatePath(mode);
+  AB200_CATCH
+}
+
+namespace {
+void digitalType(const char *what, int dtype) {
+  if (dtype != AB200_DTYPE_F32 && dtype != AB200_DTYPE_F16 && dtype != AB200_DTYPE_BF16) {
+    AB200_FATAL(what << ": unknown element type " << dtype);
+  }
+}
+void digitalRows(const char *what, long long rows, int cols, int max_cols) {
+  if (rows < 0 || rows > 0x7fffffffLL) {
+    AB200_FATAL(what << ": the number of rows must be between 0 and 2^31 - 1");
+  }
+  if (cols < 1 || cols > max_cols) {
+    AB200_FATAL(what << ": rows must have 1 to " << max_cols << " elements, got " << cols);
+  }
+}
+ab200::DropoutArgs digitalDrop(const char *what, double p, uint64_t seed, uint32_t call) {
+  if (!(p >= 0.0 && p <= 1.0)) {
+    AB200_FATAL(what << ": the dropout probability must be between 0 and 1");
+  }
+  return {p, seed, call};
+}
+void digitalPointer(const char *what, const char *name, const void *p, long long rows) {
+  if (rows > 0 && p == nullptr) {
+    AB200_FATAL(what << ": " << name << " is null");
+  }
+}
+void digitalAdapters(const char *what, long long rows, int segments, const void *starts, const void *ids, int rank,
+                     int adapters, int dtype) {
+  digitalType(what, dtype);
+  if (segments < 0 || segments > (1 << 24)) {
+    AB200_FATAL(what << ": the number of requests must be between 0 and 2^24");
+  }
+  if (starts == nullptr && segments != rows) {
+    AB200_FATAL(what << ": without row_starts there is one request per row");
+  }
+  digitalPointer(what, "adapter_ids", ids, segments);
+  if (rank < 1 || rank > ab200::kLowRankMax) {
+    AB200_FATAL(what << ": the rank must be between 1 and " << ab200::kLowRankMax << ", got " << rank);
+  }
+  if (adapters < 1 || adapters > 65535) {
+    AB200_FATAL(what << ": the number of adapters must be between 1 and 65535");
+  }
+}
+constexpr int kMaxWidth = 1 << 24;
+} // namespace
+
+int ab200_dropout(const void *x, long long x_stride, const void *residual, long long residual_stride, void *y,
+                  long long y_stride, long long rows, int cols, int dtype, double p, uint64_t seed, uint32_t call,
+                  void *stream) {
+  AB200_TRY
+  digitalType("dropout", dtype);
+  digitalRows("dropout", rows, cols, 1 << 30);
+  digitalPointer("dropout", "x", x, rows);
+  digitalPointer("dropout", "y", y, rows);
+  ab200::dropoutApply({x, x_stride}, {residual, residual_stride}, {y, y_stride}, rows, cols, dtype,
+                      digitalDrop("dropout", p, seed, call), (cudaStream_t)stream);
+  AB200_CATCH
+}
+
+int ab200_layer_norm_forward(const void *x, long long x_stride, const void *residual, long long residual_stride,
+                             const void *weight, const void *bias, void *y, long long y_stride, void *h,
+                             long long h_stride, float *mean, float *rstd, long long rows, int cols, int dtype,
+                             int param_dtype, float eps, double p, uint64_t seed, uint32_t call, void *stream) {
+  AB200_TRY
+  digitalType("layer_norm", dtype);
+  digitalType("layer_norm", param_dtype);
+  digitalRows("layer_norm", rows, cols, ab200::kNormMaxCols);
+  digitalPointer("layer_norm", "x", x, rows);
+  digitalPointer("layer_norm", "y", y, rows);
+  if ((mean == nullptr) != (rstd == nullptr)) {
+    AB200_FATAL("layer_norm: mean and rstd are wanted together or not at all");
+  }
+  ab200::NormArgs a = {{x, x_stride}, {residual, residual_stride}, {y, y_stride}, {h, h_stride}, weight, bias, mean,
+                       rstd, rows, cols, dtype, param_dtype, eps, digitalDrop("layer_norm", p, seed, call)};
+  ab200::normForward(a, (cudaStream_t)stream);
+  AB200_CATCH
+}
+
+int ab200_layer_norm_workspace(long long rows, int cols, long long *floats) {
+  AB200_TRY
+  digitalRows("layer_norm", rows, cols, ab200::kNormMaxCols);
+  digitalPointer("layer_norm_workspace", "floats", floats, 1);
+  *floats = ab200::normGradWorkspace(rows, cols);
+  AB200_CATCH
+}
+
+int ab200_layer_norm_backward(const void *gy, long long gy_stride, const void *gh, long long gh_stride, const void *x,
+                              long long x_stride, const void *residual, long long residual_stride, const void *weight, const float *mean, const float *rstd, void *dh,
+                              long long dh_stride, void *dx, long long dx_stride, void *dweight, void *dbias,
+                              float *workspace, long long rows, int cols, int dtype, int param_dtype, double p,
+                              uint64_t seed, uint32_t call, void *stream) {
+  AB200_TRY
+  digitalType("layer_norm", dtype);
+  digitalType("layer_norm", param_dtype);
+  digitalRows("layer_norm", rows, cols, ab200::kNormMaxCols);
+  digitalPointer("layer_norm", "gy", gy, rows);
+  digitalPointer("layer_norm", "x", x, rows);
+  digitalPointer("layer_norm", "mean", mean, rows);
+  digitalPointer("layer_norm", "rstd", rstd, rows);
+  const bool params = dweight != nullptr || dbias != nullptr;
+  if (params) {
+    digitalPointer("layer_norm", "workspace", workspace, rows);
+  }
+  ab200::NormGradArgs a = {{gy, gy_stride}, {gh, gh_stride}, {x, x_stride}, {residual, residual_stride}, {dh, dh_stride}, {dx, dx_stride},
+                           weight, mean, rstd, dweight, dbias, params ? workspace : nullptr, rows, cols, dtype, param_dtype,
+                           digitalDrop("layer_norm", p, seed, call)};
+  ab200::normBackward(a, (cudaStream_t)stream);
+  AB200_CATCH
+}
+
+int ab200_low_rank_apply(const void *x, long long x_stride, const void *base, long long base_stride, void *y,
+                         long long y_stride, const void *a, const void *b, const float *scale,
+                         const int32_t *adapter_ids, const int32_t *row_starts, int n_requests, long long rows, int k,
+                         int n, int rank, int n_adapters, int dtype, float *v, void *stream) {
+  AB200_TRY
+  digitalAdapters("low_rank", rows, n_requests, row_starts, adapter_ids, rank, n_adapters, dtype);
+  digitalRows("low_rank", rows, k, kMaxWidth);
+  digitalRows("low_rank", rows, n, kMaxWidth);
+  digitalPointer("low_rank", "x", x, rows);
+  digitalPointer("low_rank", "a", a, rows);
+  digitalPointer("low_rank", "scale", scale, rows);
+  if (rows > 0 && y == nullptr && v == nullptr) {
+    AB200_FATAL("low_rank: neither y nor v is wanted");
+  }
+  if (y != nullptr) {
+    digitalPointer("low_rank", "b", b, rows);
+  }
+  if (y != nullptr && y == base && y_stride != base_stride) {
+    AB200_FATAL("low_rank: y in the place of base needs base's row stride");
+  }
+  ab200::LowRankArgs args = {{row_starts, adapter_ids, n_requests, rows}, {x, x_stride}, {base, base_stride},
+                             {y, y_stride}, a, b, scale, v, k, n, rank, n_adapters, dtype};
+  ab200::lowRankApply(args, (cudaStream_t)stream);
+  AB200_CATCH
+}
+
+int ab200_low_rank_grad_workspace(long long rows, int n_requests, int one_row_each, int k, int n, int rank,
+                                  long long *bytes) {
+  AB200_TRY
+  digitalAdapters("low_rank_grad", one_row_each ? n_requests : rows, n_requests, one_row_each ? nullptr : bytes, bytes,
+                  rank, 1, AB200_DTYPE_F32);
+  digitalRows("low_rank_grad", rows, std::max(k, 1), kMaxWidth);
+  digitalRows("low_rank_grad", rows, std::max(n, 1), kMaxWidth);
+  digitalPointer("low_rank_grad_workspace", "bytes", bytes, 1);
+  *bytes = ab200::lowRankGradWorkspace(rows, n_requests, one_row_each != 0, std::max(k, 0), std::max(n, 0), rank);
+  AB200_CATCH
+}
+
+int ab200_low_rank_grad(const void *x, long long x_stride, const float *u, void *da, int k, const void *gy,
+                        long long gy_stride, const float *v, void *db, int n, const int32_t *adapter_ids,
+                        const int32_t *row_starts, int n_requests, long long rows, int rank, int n_adapters, int dtype,
+                        void *workspace, void *stream) {
+  AB200_TRY
+  digitalAdapters("low_rank_grad", rows, n_requests, row_starts, adapter_ids, rank, n_adapters, dtype);
+  if (da != nullptr) {
+    digitalRows("low_rank_grad", rows, k, kMaxWidth);
+    digitalPointer("low_rank_grad", "x", x, rows);
+    digitalPointer("low_rank_grad", "u", u, rows);
+  }
+  if (db != nullptr) {
+    digitalRows("low_rank_grad", rows, n, kMaxWidth);
+    digitalPointer("low_rank_grad", "gy", gy, rows);
+    digitalPointer("low_rank_grad", "v", v, rows);
+  }
+  digitalPointer("low_rank_grad", "workspace", workspace, rows);
+  ab200::LowRankGradArgs args = {{row_starts, adapter_ids, n_requests, rows}, {{x, x_stride}, {gy, gy_stride}}, {u, v},
+                                 {da, db}, {k, n}, workspace, rank, n_adapters, dtype};
+  ab200::lowRankGrad(args, (cudaStream_t)stream);
   AB200_CATCH
 }
 

@@ -1,0 +1,239 @@
+// Device helpers of the digital operators: element types, a warp's span of 256 neighbouring
+// elements of a row, and the counter-based keep decision of the dropout.
+#pragma once
+
+#include "common.cuh"
+#include "digital.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace ab200 {
+
+// streaming multiprocessors of the current device
+int digitalSmCount();
+
+enum : uint32_t {
+  TAG_DROPOUT = 0xB0000000u,     // high half-words of the draws
+  TAG_DROPOUT_LOW = 0xB0000001u, // low half-words, looked at only where a high one ties
+};
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <> struct Elem<__half> {
+  static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+};
+template <> struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+};
+
+// two 16-bit elements of one word
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// ---- spans ------------------------------------------------------------------------------------
+// A warp works on spans of 256 neighbouring elements of a row, eight per lane. Where every row
+// starts on the width of eight elements and the width is a multiple of eight (VEC), a lane has
+// eight neighbours, one 16-byte (16-bit types) or 32-byte (fp32, the widest load of this GPU)
+// access; elsewhere lane l has the elements l, l + 32, ..., so that single loads stay coalesced.
+// col(i) is the column of a lane's element i in both.
+template <bool VEC> struct Span {
+  static __device__ __forceinline__ int col(int span, int lane, int i) {
+    return span * 256 + (VEC ? lane * 8 + i : lane + i * 32);
+  }
+};
+
+__device__ __forceinline__ void load32B(const float *p, float v[8]) {
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+                 "=f"(v[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void store32B(float *p, const float v[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]),
+               "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+template <typename T> __device__ __forceinline__ void unpack8(const uint4 &q, float v[8]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 f = unpack2<T>(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// the eight elements of a lane as they lie in memory, so that loads can be issued long before the
+// conversion; columns past the end read as zero
+template <typename T, bool VEC> struct Raw8 {
+  uint4 q;
+  __device__ __forceinline__ void load(const T *row, int span, int lane, int cols) {
+    q = make_uint4(0, 0, 0, 0);
+    if (VEC) {
+      const int c = Span<true>::col(span, lane, 0);
+      if (c < cols) {
+        q = *reinterpret_cast<const uint4 *>(row + c);
+      }
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int c = Span<false>::col(span, lane, i);
+        if (c < cols) {
+          const uint32_t b = reinterpret_cast<const uint16_t *>(row)[c];
+          w[i >> 1] |= b << (16 * (i & 1));
+        }
+      }
+      q = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __device__ __forceinline__ void get(float v[8]) const { unpack8<T>(q, v); }
+};
+template <bool VEC> struct Raw8<float, VEC> {
+  float f[8];
+  __device__ __forceinline__ void load(const float *row, int span, int lane, int cols) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      f[i] = 0.0f;
+    }
+    if (VEC) {
+      const int c = Span<true>::col(span, lane, 0);
+      if (c < cols) {
+        load32B(row + c, f);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int c = Span<false>::col(span, lane, i);
+        if (c < cols) {
+          f[i] = row[c];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float v[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      v[i] = f[i];
+    }
+  }
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void storeSpan(T *row, int span, int lane, int cols, const float v[8]) {
+  if (VEC) {
+    const int c = Span<true>::col(span, lane, 0);
+    if (c < cols) {
+      if constexpr (sizeof(T) == 4) {
+        store32B(reinterpret_cast<float *>(row) + c, v);
+      } else {
+        uint4 q;
+        q.x = pack2<T>(v[0], v[1]);
+        q.y = pack2<T>(v[2], v[3]);
+        q.z = pack2<T>(v[4], v[5]);
+        q.w = pack2<T>(v[6], v[7]);
+        *reinterpret_cast<uint4 *>(row + c) = q;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int c = Span<false>::col(span, lane, i);
+      if (c < cols) {
+        row[c] = Elem<T>::put(v[i]);
+      }
+    }
+  }
+}
+
+// ---- dropout ----------------------------------------------------------------------------------
+// Element (row, col) is kept when a 32-bit word of its own is at least p * 2^32. The word's high
+// half is lane col % 8 of the Philox4x32-10 block (row * ceil(cols / 8) + col / 8), its low half
+// the same lane of a second block (TAG_DROPOUT_LOW), so one draw serves eight elements; the second
+// one is made only where a high half equals the threshold's (once in 2^13 blocks), which keeps the
+// probability exact to 2^-32 at half the draws that one word per element would take.
+struct DropKey {
+  uint32_t hi, lo; // halves of the threshold; hi is 65536 where everything is dropped
+  float scale;     // 1 / (1 - p)
+  uint32_t call;
+  PhiloxKey key;
+};
+inline DropKey dropKey(const DropoutArgs &d) {
+  const double t = d.p * 4294967296.0;
+  const uint64_t thr = (uint64_t)(t + 0.5);
+  DropKey k;
+  k.hi = (uint32_t)(thr >> 16);
+  k.lo = (uint32_t)(thr & 0xffffu);
+  k.scale = d.p < 1.0 ? (float)(1.0 / (1.0 - d.p)) : 0.0f;
+  k.call = d.call;
+  k.key.k0 = (uint32_t)d.seed;
+  k.key.k1 = (uint32_t)(d.seed >> 32);
+  return k;
+}
+// bit i: lane i of the block is kept
+__device__ __forceinline__ uint32_t keepBits(const DropKey &k, uint64_t block) {
+  uint32_t w[4];
+  philox4x32_10((uint32_t)block, (uint32_t)(block >> 32), k.call, TAG_DROPOUT, k.key, w);
+  uint32_t keep = 0, tie = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t h = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+    keep |= (h >= k.hi ? 1u : 0u) << i;
+    tie |= (h == k.hi ? 1u : 0u) << i;
+  }
+  if (tie != 0 && k.lo != 0) {
+    philox4x32_10((uint32_t)block, (uint32_t)(block >> 32), k.call, TAG_DROPOUT_LOW, k.key, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint32_t l = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+      keep &= ~((((tie >> i) & 1u) != 0 && l < k.lo ? 1u : 0u) << i);
+    }
+  }
+  return keep;
+}
+// bit i: element i of this lane (as Span<VEC> lays them out) is kept. Every lane of the warp draws
+// the block of its own eight neighbours; without VEC the bits are passed to the lanes that hold
+// the elements. All lanes have to call it.
+template <bool VEC>
+__device__ __forceinline__ uint32_t keepOfSpan(const DropKey &k, long long row, int span, int lane, int cols) {
+  const uint64_t blocks = (uint64_t)((cols + 7) >> 3);
+  const uint32_t mine = keepBits(k, (uint64_t)row * blocks + (uint64_t)(span * 32 + lane));
+  if (VEC) {
+    return mine;
+  }
+  uint32_t keep = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t b = __shfl_sync(0xffffffffu, mine, (lane >> 3) + 4 * i);
+    keep |= ((b >> (lane & 7)) & 1u) << i;
+  }
+  return keep;
+}
+
+// rows and width fit the accesses of eight elements
+inline bool spansAlign(const void *p, long long ld, int type) {
+  const uintptr_t bytes = type == DT_F32 ? 32 : 16;
+  return p == nullptr || ((uintptr_t)p % bytes == 0 && ld % 8 == 0);
+}
+
+} // namespace ab200

@@ -1,0 +1,503 @@
+// Layer norm, forward and backward, with the residual sum and the dropout in front of it:
+//   h = residual + drop(x);  mu = mean h;  s = (mean (h - mu)^2 + eps)^-1/2;  y = (h - mu) s w + b
+//   t = gy w;  u = (h - mu) s;  dh = s (t - mean t - u mean(t u)) + gh;  dx = drop(dh)
+//   dw = sum over rows of gy u;  db = sum over rows of gy
+// The backward pass sums h again from x and the residual rather than read the rounded one: an
+// error of 2^-9 (bf16) of h would go straight into the fp32 sums of dw.
+// Both passes are bound by memory. A row is read once and stays in registers between its two sums
+// (the squares are summed about the mean, so an offset of the row costs no digits): one warp per
+// row up to 1024 columns (WIDE false, blocks of four rows), a block per row above, whose warps hold
+// two spans of 256 columns each, four above 8192 columns (some of the backward pass's registers
+// spill there).
+// Means, sums and gradients of the parameters are held in fp32; y and h are rounded once, from the
+// unrounded sum.
+#include "digital.cuh"
+
+#include <algorithm>
+
+namespace ab200 {
+
+namespace {
+
+constexpr int kRowThreads = 128; // of blocks whose warps have rows of their own
+
+struct NormShape {
+  long long rows;
+  int cols;
+  int spans;         // of 256 columns
+  int warps_per_row; // warp w of a row has the spans w, w + warps_per_row, ...
+  int rows_per_block;
+  float inv_cols;
+};
+
+__device__ __forceinline__ float warpSum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
+  return v;
+}
+// sum over the warps of a row; `red` has a slot per warp, used in turn so that one barrier per sum
+// is enough
+template <bool WIDE> __device__ __forceinline__ float rowSum(float v, int warps, float *red) {
+  v = warpSum(v);
+  if (WIDE) {
+    if ((threadIdx.x & 31) == 0) {
+      red[threadIdx.x >> 5] = v;
+    }
+    __syncthreads();
+    v = 0.0f;
+    for (int w = 0; w < warps; w++) {
+      v += red[w];
+    }
+  }
+  return v;
+}
+template <bool WIDE>
+__device__ __forceinline__ float2 rowSum2(float a, float b, int warps, float2 *red) {
+  a = warpSum(a);
+  b = warpSum(b);
+  if (WIDE) {
+    if ((threadIdx.x & 31) == 0) {
+      red[threadIdx.x >> 5] = make_float2(a, b);
+    }
+    __syncthreads();
+    a = b = 0.0f;
+    for (int w = 0; w < warps; w++) {
+      const float2 t = red[w];
+      a += t.x;
+      b += t.y;
+    }
+  }
+  return make_float2(a, b);
+}
+
+// parameters are read per row, from L1 after the first row of an SM
+template <bool VEC>
+__device__ __forceinline__ void loadParam(const void *p, int w_type, float none, int span, int lane, int cols,
+                                          float v[8]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      v[i] = none;
+    }
+    return;
+  }
+  if (w_type == DT_F32) {
+    Raw8<float, VEC> r;
+    r.load((const float *)p, span, lane, cols);
+    r.get(v);
+  } else if (w_type == DT_F16) {
+    Raw8<__half, VEC> r;
+    r.load((const __half *)p, span, lane, cols);
+    r.get(v);
+  } else {
+    Raw8<__nv_bfloat16, VEC> r;
+    r.load((const __nv_bfloat16 *)p, span, lane, cols);
+    r.get(v);
+  }
+}
+
+struct NormFwd {
+  const void *x, *res, *w, *b;
+  void *y, *h;
+  float *mean, *rstd;
+  long long x_ld, res_ld, y_ld, h_ld;
+  int w_type;
+  float eps;
+  int drop;
+};
+
+template <typename T, bool VEC, bool WIDE, int NS>
+__global__ void __launch_bounds__(WIDE ? 512 : kRowThreads)
+    normForwardKernel(NormFwd a, NormShape sh, DropKey key) {
+  pdlEnter();
+  __shared__ float red[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int w0 = WIDE ? warp : 0;
+  const long long row = (long long)blockIdx.x * sh.rows_per_block + (WIDE ? 0 : warp);
+  if (row >= sh.rows) {
+    return; // only whole warps of rows of their own
+  }
+  const T *xr = (const T *)a.x + row * a.x_ld;
+  float v[NS][8];
+  {
+    Raw8<T, VEC> rx[NS], rr[NS];
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      rx[s].load(xr, w0 + s * sh.warps_per_row, lane, sh.cols);
+    }
+    if (a.res) {
+      const T *rrow = (const T *)a.res + row * a.res_ld;
+#pragma unroll
+      for (int s = 0; s < NS; s++) {
+        rr[s].load(rrow, w0 + s * sh.warps_per_row, lane, sh.cols);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      rx[s].get(v[s]);
+      if (a.drop) {
+        const uint32_t keep = keepOfSpan<VEC>(key, row, w0 + s * sh.warps_per_row, lane, sh.cols);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          v[s][i] = (keep >> i) & 1u ? v[s][i] * key.scale : 0.0f;
+        }
+      }
+      if (a.res) {
+        float r[8];
+        rr[s].get(r);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          v[s][i] += r[i];
+        }
+      }
+    }
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      sum += v[s][i]; // columns past the end hold zeros
+    }
+  }
+  const float mean = rowSum<WIDE>(sum, sh.warps_per_row, red[0]) * sh.inv_cols;
+  float sq = 0.0f;
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float d = v[s][i] - mean;
+      sq += Span<VEC>::col(w0 + s * sh.warps_per_row, lane, i) < sh.cols ? d * d : 0.0f;
+    }
+  }
+  const float var = rowSum<WIDE>(sq, sh.warps_per_row, red[1]) * sh.inv_cols;
+  const float rstd = rsqrtf(var + a.eps);
+  if (a.mean != nullptr && lane == 0 && w0 == 0) {
+    a.mean[row] = mean;
+    a.rstd[row] = rstd;
+  }
+  T *yr = (T *)a.y + row * a.y_ld;
+  T *hr = (T *)a.h + row * a.h_ld;
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+    const int span = w0 + s * sh.warps_per_row;
+    float w[8], b[8];
+    loadParam<VEC>(a.w, a.w_type, 1.0f, span, lane, sh.cols, w);
+    loadParam<VEC>(a.b, a.w_type, 0.0f, span, lane, sh.cols, b);
+    if (a.h) {
+      storeSpan<T, VEC>(hr, span, lane, sh.cols, v[s]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      w[i] = fmaf((v[s][i] - mean) * rstd, w[i], b[i]);
+    }
+    storeSpan<T, VEC>(yr, span, lane, sh.cols, w);
+  }
+}
+
+struct NormBwd {
+  const void *gy, *gh, *x, *res, *w;
+  void *dh, *dx;
+  const float *mean, *rstd;
+  float *partial; // [blocks][2][cols]
+  long long gy_ld, gh_ld, x_ld, res_ld, dh_ld, dx_ld;
+  int w_type;
+  int drop; // x is dropped before the sum
+};
+
+// Blocks walk over the rows with a fixed stride and keep the sums of the parameters' gradients of
+// their columns in registers; a second kernel adds the blocks' sums in order, so the result does
+// not depend on which block ran when.
+template <typename T, bool VEC, bool WIDE, int NS>
+__global__ void __launch_bounds__(WIDE ? 512 : kRowThreads)
+    normBackwardKernel(NormBwd a, NormShape sh, DropKey key) {
+  pdlEnter();
+  __shared__ float2 red[2][32];
+  extern __shared__ float join[]; // [2][cols] where a block has several rows
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int w0 = WIDE ? warp : 0;
+  float dw[NS][8], db[NS][8];
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      dw[s][i] = db[s][i] = 0.0f;
+    }
+  }
+  const long long stride = (long long)gridDim.x * sh.rows_per_block;
+  int turn = 0;
+  for (long long row = (long long)blockIdx.x * sh.rows_per_block + (WIDE ? 0 : warp);
+       row < sh.rows; row += stride) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float u[NS][8], t[NS][8];
+    Raw8<T, VEC> rx[NS], rr[NS], rg[NS], ra[NS];
+    uint32_t keep[NS];
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      const int span = w0 + s * sh.warps_per_row;
+      rx[s].load((const T *)a.x + row * a.x_ld, span, lane, sh.cols);
+      rg[s].load((const T *)a.gy + row * a.gy_ld, span, lane, sh.cols);
+    }
+    if (a.res) {
+#pragma unroll
+      for (int s = 0; s < NS; s++) {
+        rr[s].load((const T *)a.res + row * a.res_ld, w0 + s * sh.warps_per_row, lane, sh.cols);
+      }
+    }
+    if (a.gh) {
+#pragma unroll
+      for (int s = 0; s < NS; s++) {
+        ra[s].load((const T *)a.gh + row * a.gh_ld, w0 + s * sh.warps_per_row, lane, sh.cols);
+      }
+    }
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      const int span = w0 + s * sh.warps_per_row;
+      float w[8], g[8];
+      loadParam<VEC>(a.w, a.w_type, 1.0f, span, lane, sh.cols, w);
+      rx[s].get(u[s]);
+      rg[s].get(g);
+      keep[s] = 0xffu;
+      if (a.drop || a.dx) {
+        keep[s] = keepOfSpan<VEC>(key, row, span, lane, sh.cols);
+      }
+      if (a.drop) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          u[s][i] = (keep[s] >> i) & 1u ? u[s][i] * key.scale : 0.0f;
+        }
+      }
+      if (a.res) {
+        float r[8];
+        rr[s].get(r);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          u[s][i] += r[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        // a column past the end has gy = 0 and takes part in no sum
+        u[s][i] = (u[s][i] - mean) * rstd;
+        dw[s][i] = Span<VEC>::col(span, lane, i) < sh.cols ? fmaf(g[i], u[s][i], dw[s][i]) : 0.0f;
+        db[s][i] += g[i];
+        t[s][i] = g[i] * w[i];
+        s1 += t[s][i];
+        s2 = Span<VEC>::col(span, lane, i) < sh.cols ? fmaf(t[s][i], u[s][i], s2) : s2;
+      }
+    }
+    const float2 sums = rowSum2<WIDE>(s1, s2, sh.warps_per_row, red[turn & 1]);
+    turn++;
+    const float m1 = sums.x * sh.inv_cols, m2 = sums.y * sh.inv_cols;
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      const int span = w0 + s * sh.warps_per_row;
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        d[i] = rstd * (t[s][i] - m1 - u[s][i] * m2);
+      }
+      if (a.gh) {
+        float g[8];
+        ra[s].get(g);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          d[i] += g[i];
+        }
+      }
+      if (a.dh) {
+        storeSpan<T, VEC>((T *)a.dh + row * a.dh_ld, span, lane, sh.cols, d);
+      }
+      if (a.dx) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          d[i] = (keep[s] >> i) & 1u ? d[i] * key.scale : 0.0f;
+        }
+        storeSpan<T, VEC>((T *)a.dx + row * a.dx_ld, span, lane, sh.cols, d);
+      }
+    }
+  }
+  if (a.partial == nullptr) {
+    return;
+  }
+  float *out = a.partial + (long long)blockIdx.x * 2 * sh.cols;
+  if (!WIDE) {
+    // the block's warps have the same columns: they add up one after the other
+    const int n_warps = blockDim.x >> 5;
+    for (int w = 0; w < n_warps; w++) {
+      if (warp == w) {
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int c = Span<VEC>::col(s, lane, i);
+            if (c < sh.cols) {
+              const float pw = w > 0 ? join[c] : 0.0f, pb = w > 0 ? join[sh.cols + c] : 0.0f;
+              (w + 1 < n_warps ? join : out)[c] = pw + dw[s][i];
+              (w + 1 < n_warps ? join : out)[sh.cols + c] = pb + db[s][i];
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      const int span = w0 + s * sh.warps_per_row;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int c = Span<VEC>::col(span, lane, i);
+        if (c < sh.cols) {
+          out[c] = dw[s][i];
+          out[sh.cols + c] = db[s][i];
+        }
+      }
+    }
+  }
+}
+
+// dw[c] / db[c] = sum over the blocks' partial sums; 32 columns x 32 parts of the blocks per CTA
+__global__ void __launch_bounds__(1024)
+    normParamKernel(const float *__restrict__ partial, int blocks, int cols, void *dw, void *db, int w_type) {
+  pdlEnter();
+  __shared__ float part[32][33];
+  const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane; // over [dw, db]
+  float sum = 0.0f;
+  if (c < 2 * cols) {
+#pragma unroll 4
+    for (int b = q; b < blocks; b += 32) {
+      sum += partial[(long long)b * 2 * cols + c];
+    }
+  }
+  part[q][lane] = sum;
+  __syncthreads();
+  sum = warpSum(part[lane][q]);
+  const int col = blockIdx.x * 32 + q;
+  if (lane == 0 && col < 2 * cols) {
+    void *dst = col < cols ? dw : db;
+    const int e = col < cols ? col : col - cols;
+    if (dst != nullptr) {
+      if (w_type == DT_F32) {
+        ((float *)dst)[e] = sum;
+      } else if (w_type == DT_F16) {
+        ((__half *)dst)[e] = __float2half_rn(sum);
+      } else {
+        ((__nv_bfloat16 *)dst)[e] = __float2bfloat16_rn(sum);
+      }
+    }
+  }
+}
+
+NormShape normShape(long long rows, int cols) {
+  NormShape sh;
+  sh.rows = rows;
+  sh.cols = cols;
+  sh.spans = (cols + 255) / 256;
+  sh.warps_per_row = sh.spans <= 4 ? 1 : sh.spans <= 32 ? (sh.spans + 1) / 2 : (sh.spans + 3) / 4;
+  sh.rows_per_block = sh.spans <= 4 ? kRowThreads / 32 : 1;
+  sh.inv_cols = 1.0f / (float)cols;
+  return sh;
+}
+int normThreads(const NormShape &sh) { return sh.spans <= 4 ? kRowThreads : sh.warps_per_row * 32; }
+
+// blocks of the backward pass: sixteen warps to a multiprocessor, fewer where rows are few
+int normGradBlocks(const NormShape &sh) {
+  const long long resident = std::max(1, 16 / (normThreads(sh) / 32));
+  return (int)std::max(1LL, std::min((sh.rows + sh.rows_per_block - 1) / sh.rows_per_block,
+                                     resident * digitalSmCount()));
+}
+
+template <template <typename, bool, bool, int> class Launch, typename T, bool VEC, typename... Args>
+void normDispatchShape(const NormShape &sh, Args &&...args) {
+  switch (sh.spans) {
+  case 1: Launch<T, VEC, false, 1>::run(sh, args...); break;
+  case 2: Launch<T, VEC, false, 2>::run(sh, args...); break;
+  case 3: Launch<T, VEC, false, 3>::run(sh, args...); break;
+  case 4: Launch<T, VEC, false, 4>::run(sh, args...); break;
+  default:
+    if (sh.spans <= 32) {
+      Launch<T, VEC, true, 2>::run(sh, args...);
+    } else {
+      Launch<T, VEC, true, 4>::run(sh, args...);
+    }
+  }
+}
+template <template <typename, bool, bool, int> class Launch, typename... Args>
+void normDispatch(int type, bool vec, const NormShape &sh, Args &&...args) {
+  switch (type) {
+  case DT_F32:
+    vec ? normDispatchShape<Launch, float, true>(sh, args...) : normDispatchShape<Launch, float, false>(sh, args...);
+    break;
+  case DT_F16:
+    vec ? normDispatchShape<Launch, __half, true>(sh, args...)
+        : normDispatchShape<Launch, __half, false>(sh, args...);
+    break;
+  default:
+    vec ? normDispatchShape<Launch, __nv_bfloat16, true>(sh, args...)
+        : normDispatchShape<Launch, __nv_bfloat16, false>(sh, args...);
+  }
+}
+
+template <typename T, bool VEC, bool WIDE, int NS> struct LaunchForward {
+  static void run(const NormShape &sh, const NormFwd &a, const DropKey &key, cudaStream_t stream) {
+    const long long blocks = (sh.rows + sh.rows_per_block - 1) / sh.rows_per_block;
+    AB200_CUDA(launchChained(normForwardKernel<T, VEC, WIDE, NS>, dim3((unsigned)blocks), dim3(normThreads(sh)), 0, stream, a,
+                             sh, key));
+    AB200_LAUNCH_CHECK();
+  }
+};
+template <typename T, bool VEC, bool WIDE, int NS> struct LaunchBackward {
+  static void run(const NormShape &sh, const NormBwd &a, const DropKey &key, int blocks, cudaStream_t stream) {
+    const size_t smem = a.partial && !WIDE ? (size_t)sh.cols * 2 * sizeof(float) : 0;
+    AB200_CUDA(launchChained(normBackwardKernel<T, VEC, WIDE, NS>, dim3((unsigned)blocks), dim3(normThreads(sh)), smem, stream,
+                             a, sh, key));
+    AB200_LAUNCH_CHECK();
+  }
+};
+
+} // namespace
+
+void normForward(const NormArgs &a, cudaStream_t stream) {
+  if (a.rows <= 0) {
+    return;
+  }
+  const NormShape sh = normShape(a.rows, a.cols);
+  const bool vec = a.cols % 8 == 0 && spansAlign(a.x.p, a.x.ld, a.type) &&
+                   spansAlign(a.residual.p, a.residual.ld, a.type) && spansAlign(a.y.p, a.y.ld, a.type) &&
+                   spansAlign(a.h.p, a.h.ld, a.type) && spansAlign(a.weight, 0, a.w_type) &&
+                   spansAlign(a.bias, 0, a.w_type);
+  NormFwd k = {a.x.p,     a.residual.p,  a.weight, a.bias,  a.y.p,    a.h.p, a.mean, a.rstd, a.x.ld,
+               a.residual.ld, a.y.ld, a.h.ld,   a.w_type, a.eps, a.drop.p > 0.0};
+  normDispatch<LaunchForward>(a.type, vec, sh, k, dropKey(a.drop), stream);
+}
+
+long long normGradWorkspace(long long rows, int cols) {
+  return rows <= 0 ? 0 : (long long)normGradBlocks(normShape(rows, cols)) * 2 * cols;
+}
+
+void normBackward(const NormGradArgs &a, cudaStream_t stream) {
+  const NormShape sh = normShape(a.rows, a.cols);
+  const int blocks = a.rows > 0 ? normGradBlocks(sh) : 0;
+  if (blocks > 0) {
+    const bool vec = a.cols % 8 == 0 && spansAlign(a.gy.p, a.gy.ld, a.type) && spansAlign(a.gh.p, a.gh.ld, a.type) &&
+                     spansAlign(a.x.p, a.x.ld, a.type) && spansAlign(a.residual.p, a.residual.ld, a.type) &&
+                     spansAlign(a.dh.p, a.dh.ld, a.type) && spansAlign(a.dx.p, a.dx.ld, a.type) &&
+                     spansAlign(a.weight, 0, a.w_type);
+    NormBwd k = {a.gy.p,    a.gh.p,  a.x.p,   a.residual.p,  a.weight,  a.dh.p,  a.dx.p,   a.mean,
+                 a.rstd,    a.partial, a.gy.ld, a.gh.ld, a.x.ld, a.residual.ld, a.dh.ld, a.dx.ld,
+                 a.w_type, a.residual.p != nullptr && a.drop.p > 0.0};
+    normDispatch<LaunchBackward>(a.type, vec, sh, k, dropKey(a.drop), blocks, stream);
+  }
+  if (a.dweight || a.dbias) {
+    AB200_CUDA(launchChained(normParamKernel, dim3((unsigned)((2 * a.cols + 31) / 32)), dim3(1024), 0, stream,
+                             (const float *)a.partial, blocks, a.cols, a.dweight, a.dbias, a.w_type));
+    AB200_LAUNCH_CHECK();
+  }
+}
+
+} // namespace ab200

@@ -787,6 +787,77 @@ int ab200_mvm_forward_noalloc(const ab200_io_params *forward_io, const float *w_
                               int x_size, int d_size, const float *x_dev, float *d_dev,
                               int m_batch, uint64_t seed, uint32_t call, void *stream);
 
+/* ---- digital operators around the tiles of a transformer block -----------------------------------
+ * No counterpart in the reference, where they are torch calls. Conductances are written once, so a
+ * model on analog tiles is adapted digitally: by low-rank adapters beside the tiles, with layer norms and
+ * dropout around them. All pointers are device memory of the CURRENT device, `stream` one of its streams.
+ * Matrices are rows of neighbouring elements, a row's start `*_stride` elements behind the one before
+ * (a stride of 0 repeats one row and is for inputs only). Nothing is allocated and nothing is waited
+ * for; the calls can be captured into a graph. Sums, means and saved values are fp32 whatever the type,
+ * results are rounded once. Outputs must not overlap inputs unless a call says so. */
+enum ab200_dtype { AB200_DTYPE_F32 = 0, AB200_DTYPE_F16 = 1, AB200_DTYPE_BF16 = 2 };
+
+/* y = keep ? x / (1 - p) : 0, plus `residual` where it is not null. A dropped element is 0 whatever it
+ * held. Which elements are kept is a function of (seed, call, row, column, number of columns) alone: element (r, c)
+ * is kept when a 32-bit word is at least round(p * 2^32); the word's high half is half-word c % 8 of
+ * the Philox4x32-10 block r * ceil(cols / 8) + c / 8 (counter: block, call, 0xB0000000; key: seed), its
+ * low half the same half-word of the block with 0xB0000001. So no mask is stored: the gradient is
+ * the same call on the incoming gradient. y may be x or residual. */
+int ab200_dropout(const void *x, long long x_stride, const void *residual, long long residual_stride,
+                  void *y, long long y_stride, long long rows, int cols, int dtype, double p,
+                  uint64_t seed, uint32_t call, void *stream);
+
+/* h = residual + dropout(x) (either part may be missing: residual null, p = 0);
+ * y = (h - mean(h)) * rstd(h) * weight + bias, rstd = (variance + eps)^-1/2, rows of at most 16384 elements.
+ * weight and bias [cols] are of param_dtype and may be null (1 and 0); h (may be null) receives the sum,
+ * mean and rstd [rows] (both null or neither) what the backward pass reads. y and h are rounded from the
+ * same fp32 sum. y or h may be x or residual, but not the same one.
+ * backward: gy, gh (may be null) are the gradients of y and of h. x and residual are what the forward pass
+ * read, and h is summed again in fp32; with residual null, x is h itself (fp32 callers may keep h instead
+ * of the two). dh (may be null) receives the gradient of h (which is the residual's), dx (may be
+ * null) the same behind the dropout; dweight
+ * and dbias [cols] (each may be null) are of param_dtype; where one is wanted, workspace has the floats
+ * that ab200_layer_norm_workspace gives. The sums over rows are added in a fixed order. */
+int ab200_layer_norm_forward(const void *x, long long x_stride, const void *residual,
+                             long long residual_stride, const void *weight, const void *bias, void *y,
+                             long long y_stride, void *h, long long h_stride, float *mean, float *rstd,
+                             long long rows, int cols, int dtype, int param_dtype, float eps, double p,
+                             uint64_t seed, uint32_t call, void *stream);
+int ab200_layer_norm_workspace(long long rows, int cols, long long *floats);
+int ab200_layer_norm_backward(const void *gy, long long gy_stride, const void *gh, long long gh_stride,
+                              const void *x, long long x_stride, const void *residual,
+                              long long residual_stride, const void *weight, const float *mean,
+                              const float *rstd, void *dh, long long dh_stride, void *dx,
+                              long long dx_stride, void *dweight, void *dbias, float *workspace,
+                              long long rows, int cols, int dtype, int param_dtype, double p,
+                              uint64_t seed, uint32_t call, void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection. Request j has the rows
+ * [row_starts[j], row_starts[j + 1]) (device memory, n_requests + 1 values that do not decrease; null: request
+ * j is row j) and the adapter adapter_ids[j]; an id outside [0, n_adapters) means none. With a
+ * [n_adapters][rank][k], b [n_adapters][rank][n] (contiguous), scale [n_adapters], rank at most 256:
+ *   y = base + (scale x a^T) b   for rows with an adapter,   y = base   for all others;
+ * base null counts as zero; y may be base (rows without an adapter are then not touched).
+ * v [rows][rank] (may be null) receives scale x a^T of the rows with an adapter; y may be null then.
+ * The gradient of x is the same call on gy with a and b (k and n) exchanged, its v what the
+ * gradient of a needs (u below).
+ * grad: da = sum over an adapter's rows of u^T x, db = sum of v^T gy, of the type of x and gy, zero for
+ * adapters without rows; each may be null. workspace has the bytes that ab200_low_rank_grad_workspace
+ * gives for the same sizes (k or n 0 where that gradient is not wanted; one_row_each: row_starts is null).
+ * Requests may share an adapter; sums over rows are added in the order of the rows. Rows of one adapter
+ * cost least as one request: each request has tiles of its own. */
+int ab200_low_rank_apply(const void *x, long long x_stride, const void *base, long long base_stride,
+                         void *y, long long y_stride, const void *a, const void *b, const float *scale,
+                         const int32_t *adapter_ids, const int32_t *row_starts, int n_requests,
+                         long long rows, int k, int n, int rank, int n_adapters, int dtype, float *v,
+                         void *stream);
+int ab200_low_rank_grad_workspace(long long rows, int n_requests, int one_row_each, int k, int n, int rank,
+                                  long long *bytes);
+int ab200_low_rank_grad(const void *x, long long x_stride, const float *u, void *da, int k, const void *gy,
+                        long long gy_stride, const float *v, void *db, int n, const int32_t *adapter_ids,
+                        const int32_t *row_starts, int n_requests, long long rows, int rank,
+                        int n_adapters, int dtype, void *workspace, void *stream);
+
 /* Kernel selection for the MVM (no counterpart in the reference, which always calls cuBLAS):
  * 0 = automatic (tensor cores for large aligned problems), 1 = CUDA cores only, 2 = tensor
  * cores whenever the IO settings allow, 3 = as 2 but never the kernel variant that pairs two
