@@ -172,62 +172,122 @@ __device__ __forceinline__ void storeSpan(T *row, int span, int lane, int cols, 
 // the same lane of a second block (TAG_DROPOUT_LOW), so one draw serves eight elements; the second
 // one is made only where a high half equals the threshold's (once in 2^13 blocks), which keeps the
 // probability exact to 2^-32 at half the draws that one word per element would take.
+//
+// The decision is taken two half-words at a time: bit 15 and bit 31 of a word of Kept say whether
+// its two elements stay, and a byte permutation spreads them into masks. With 16-bit rows the whole
+// GPU's integer pipe is what a dropout costs (Philox and 8 comparisons one by one: 75 % of that pipe, 80 us at
+// 16384 x 4096 bf16), so every instruction here shows.
 struct DropKey {
-  uint32_t hi, lo; // halves of the threshold; hi is 65536 where everything is dropped
-  float scale;     // 1 / (1 - p)
+  uint32_t hi2; // the high half of the threshold, twice
+  uint32_t lo;  // its low half; 65536 (with hi 65535) where everything is dropped
+  float scale;  // 1 / (1 - p)
   uint32_t call;
-  PhiloxKey key;
+  uint32_t a[10], b[10]; // Philox's keys of the ten rounds, which instructions take from constant memory
 };
 inline DropKey dropKey(const DropoutArgs &d) {
-  const double t = d.p * 4294967296.0;
-  const uint64_t thr = (uint64_t)(t + 0.5);
+  const uint64_t thr = (uint64_t)(d.p * 4294967296.0 + 0.5);
+  const bool all = thr >> 32 != 0;
+  const uint32_t hi = all ? 0xffffu : (uint32_t)(thr >> 16);
   DropKey k;
-  k.hi = (uint32_t)(thr >> 16);
-  k.lo = (uint32_t)(thr & 0xffffu);
+  k.hi2 = hi | hi << 16;
+  k.lo = all ? 0x10000u : (uint32_t)(thr & 0xffffu);
   k.scale = d.p < 1.0 ? (float)(1.0 / (1.0 - d.p)) : 0.0f;
   k.call = d.call;
-  k.key.k0 = (uint32_t)d.seed;
-  k.key.k1 = (uint32_t)(d.seed >> 32);
+  for (uint32_t r = 0; r < 10; r++) {
+    k.a[r] = (uint32_t)d.seed + r * 0x9E3779B9u;
+    k.b[r] = (uint32_t)(d.seed >> 32) + r * 0xBB67AE85u;
+  }
   return k;
 }
-// bit i: lane i of the block is kept
-__device__ __forceinline__ uint32_t keepBits(const DropKey &k, uint64_t block) {
-  uint32_t w[4];
-  philox4x32_10((uint32_t)block, (uint32_t)(block >> 32), k.call, TAG_DROPOUT, k.key, w);
-  uint32_t keep = 0, tie = 0;
+__device__ __forceinline__ void dropWords(const DropKey &k, uint64_t block, uint32_t tag, uint32_t out[4]) {
+  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = k.call, c3 = tag;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const uint32_t h = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
-    keep |= (h >= k.hi ? 1u : 0u) << i;
-    tie |= (h == k.hi ? 1u : 0u) << i;
+  for (int r = 0; r < 10; r++) { // philox4x32_10 with the keys at hand
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k.a[r];
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k.b[r];
+    c1 = (uint32_t)p1;
+    c3 = (uint32_t)p0;
   }
-  if (tie != 0 && k.lo != 0) {
-    philox4x32_10((uint32_t)block, (uint32_t)(block >> 32), k.call, TAG_DROPOUT_LOW, k.key, w);
+  out[0] = c0;
+  out[1] = c1;
+  out[2] = c2;
+  out[3] = c3;
+}
+// Bits 15 and 31 of word i: half-words 0 and 1 of the block's word i (elements 2 i and 2 i + 1) stay;
+// the other bits mean nothing.
+struct Kept {
+  uint32_t w[4];
+};
+__device__ __forceinline__ Kept keepBlock(const DropKey &k, uint64_t block) {
+  constexpr uint32_t H = 0x80008000u;
+  uint32_t w[4];
+  dropWords(k, block, TAG_DROPOUT, w);
+  Kept kept;
+  uint32_t differ[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const uint32_t l = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
-      keep &= ~((((tie >> i) & 1u) != 0 && l < k.lo ? 1u : 0u) << i);
+  for (int i = 0; i < 4; i++) {
+    // unsigned w >= hi in each half: the low 15 bits by a subtraction that cannot borrow from the
+    // other half, the top bits where they differ
+    const uint32_t low = (w[i] | H) - (k.hi2 & ~H);
+    differ[i] = w[i] ^ k.hi2;
+    kept.w[i] = (w[i] & ~k.hi2) | (~differ[i] & low);
+  }
+  // a half-word of `differ` that is zero is a tie (the borrow of one may name the other's as well)
+  uint32_t tie = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    tie |= (differ[i] - 0x00010001u) & ~differ[i];
+  }
+  if ((tie & H) != 0 && k.lo != 0) {
+    uint32_t l[4];
+    dropWords(k, block, TAG_DROPOUT_LOW, l);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if ((differ[i] & 0xffffu) == 0 && (l[i] & 0xffffu) < k.lo) {
+        kept.w[i] &= ~0x8000u;
+      }
+      if (differ[i] >> 16 == 0 && l[i] >> 16 < k.lo) {
+        kept.w[i] &= ~0x80000000u;
+      }
     }
   }
-  return keep;
+  return kept;
 }
-// bit i: element i of this lane (as Span<VEC> lays them out) is kept. Every lane of the warp draws
-// the block of its own eight neighbours; without VEC the bits are passed to the lanes that hold
-// the elements. All lanes have to call it.
+// byte selectors with their top bit set repeat the sign of the byte (the CUDA intrinsic drops that bit)
+__device__ __forceinline__ uint32_t signMask(uint32_t w, uint32_t selectors) {
+  uint32_t m;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(m) : "r"(w), "r"(selectors));
+  return m;
+}
+// The same for the elements that a lane holds of a span. Every lane of the warp draws the block of
+// its own eight neighbours; without VEC the bits are passed to the lanes that hold the elements, and
+// element i of a lane is again bit 15 (i even) or 31 of word i / 2. All lanes have to call it.
 template <bool VEC>
-__device__ __forceinline__ uint32_t keepOfSpan(const DropKey &k, long long row, int span, int lane, int cols) {
+__device__ __forceinline__ Kept keepOfSpan(const DropKey &k, long long row, int span, int lane, int cols) {
   const uint64_t blocks = (uint64_t)((cols + 7) >> 3);
-  const uint32_t mine = keepBits(k, (uint64_t)row * blocks + (uint64_t)(span * 32 + lane));
-  if (VEC) {
-    return mine;
+  Kept mine = keepBlock(k, (uint64_t)row * blocks + (uint64_t)(span * 32 + lane));
+  if (!VEC) {
+    constexpr uint32_t H = 0x80008000u;
+    // half-word j of the block at bit 12 + j / 2 + 16 (j odd)
+    const uint32_t all = ((mine.w[0] & H) >> 3) | ((mine.w[1] & H) >> 2) | ((mine.w[2] & H) >> 1) | (mine.w[3] & H);
+    const int at = 12 + ((lane & 7) >> 1) + 16 * (lane & 1);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint32_t b = (__shfl_sync(0xffffffffu, all, (lane >> 3) + 4 * i) >> at) & 1u;
+      mine.w[i >> 1] = (i & 1) ? mine.w[i >> 1] | b << 31 : b << 15;
+    }
   }
-  uint32_t keep = 0;
+  return mine;
+}
+// v = kept ? v * scale : 0, whatever v is
+__device__ __forceinline__ void dropSpan(const DropKey &k, const Kept &kept, float v[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const uint32_t b = __shfl_sync(0xffffffffu, mine, (lane >> 3) + 4 * i);
-    keep |= ((b >> (lane & 7)) & 1u) << i;
+    // the bit, 32 times
+    const uint32_t mask = signMask(kept.w[i >> 1], (i & 1) ? 0xbbbb : 0x9999);
+    v[i] = __uint_as_float(__float_as_uint(v[i] * k.scale) & mask);
   }
-  return keep;
 }
 
 // rows and width fit the accesses of eight elements

@@ -3,6 +3,7 @@
 #include "digital.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ab200 {
 
@@ -23,26 +24,32 @@ int digitalSmCount() {
 
 namespace {
 
-// A warp takes one span of 256 elements at a time, two in flight.
-template <typename T, bool VEC, bool RES>
+// A warp takes one span of 256 elements at a time, two in flight. FLAT: the rows follow each other
+// without a gap and their blocks of eight are numbered alike, so they are one row of up to 2^30 elements.
+template <typename T, bool VEC, bool RES, bool FLAT>
 __global__ void __launch_bounds__(256)
-    dropoutKernel(const T *x, long long x_ld, const T *res, long long res_ld,
-                  T *y, long long y_ld, long long rows, int cols, DropKey key) {
+    dropoutKernel(const T *x, long long x_ld, const T *res, long long res_ld, T *y, long long y_ld, long long rows,
+                  int cols, DropKey key) {
+  using Index = typename std::conditional<FLAT, uint32_t, long long>::type;
   pdlEnter();
   const int lane = threadIdx.x & 31;
-  const int spans = (cols + 255) / 256;
-  const long long total = rows * spans;
-  const long long warps = (long long)gridDim.x * (blockDim.x / 32);
-  for (long long s = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; s < total; s += 2 * warps) {
+  const uint32_t spans = ((uint32_t)cols + 255u) / 256u;
+  const Index total = FLAT ? (Index)spans : (Index)(rows * spans);
+  const Index warps = (Index)gridDim.x * (blockDim.x / 32);
+  for (Index s = (Index)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; s < total; s += 2 * warps) {
     Raw8<T, VEC> raw[2], add[2];
     long long row[2];
     int span[2];
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      const long long t = s + q * warps;
-      // past the last span: behind the end of row 0, where nothing is read or written
-      row[q] = rows == 1 || t >= total ? 0 : total <= 0x7fffffffLL ? (uint32_t)t / (uint32_t)spans : t / spans;
-      span[q] = t < total ? (int)(t - row[q] * spans) : spans;
+      const Index t = s + q * warps;
+      if (FLAT) {
+        row[q] = 0;
+        span[q] = (int)min((uint32_t)t, spans); // past the last span nothing is read or written
+      } else {
+        row[q] = t >= total ? 0 : total <= 0x7fffffffLL ? (uint32_t)t / spans : t / spans;
+        span[q] = t < total ? (int)(t - row[q] * spans) : (int)spans;
+      }
       raw[q].load(x + row[q] * x_ld, span[q], lane, cols);
       if (RES) {
         add[q].load(res + row[q] * res_ld, span[q], lane, cols);
@@ -50,69 +57,77 @@ __global__ void __launch_bounds__(256)
     }
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      float v[8], r[8];
-      const uint32_t keep = keepOfSpan<VEC>(key, row[q], span[q], lane, cols);
+      float v[8];
+      const Kept kept = keepOfSpan<VEC>(key, row[q], span[q], lane, cols);
       raw[q].get(v);
-      if (RES) {
-        add[q].get(r);
-      }
+      if constexpr (VEC && !RES && sizeof(T) == 2) {
+        // pairs of results are masked as they are stored, a quarter of the masks
+        const int c = Span<true>::col(span[q], lane, 0);
+        if (c < cols) {
+          uint32_t o[4];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        // a dropped element is zero whatever it held, infinities and NaN included
-        v[i] = (keep >> i) & 1u ? v[i] * key.scale : 0.0f;
-        if (RES) {
-          v[i] += r[i];
+          for (int i = 0; i < 4; i++) {
+            o[i] = pack2<T>(v[2 * i] * key.scale, v[2 * i + 1] * key.scale) & signMask(kept.w[i], 0xbb99);
+          }
+          *reinterpret_cast<uint4 *>(y + row[q] * y_ld + c) = make_uint4(o[0], o[1], o[2], o[3]);
         }
+      } else {
+        dropSpan(key, kept, v);
+        if (RES) {
+          float r[8];
+          add[q].get(r);
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            v[i] += r[i];
+          }
+        }
+        storeSpan<T, VEC>(y + row[q] * y_ld, span[q], lane, cols, v);
       }
-      storeSpan<T, VEC>(y + row[q] * y_ld, span[q], lane, cols, v);
     }
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool RES, bool FLAT>
 void launchDropout(RowsIn x, RowsIn residual, RowsOut y, long long rows, int cols, const DropKey &key,
                    cudaStream_t stream) {
-  const long long total = rows * ((cols + 255) / 256);
+  const long long total = rows * (((long long)cols + 255) / 256);
   const long long want = (total + 15) / 16;
   const dim3 grid((unsigned)std::max(1LL, std::min(want, (long long)digitalSmCount() * 32)));
-  if (residual.p) {
-    AB200_CUDA(launchChained(dropoutKernel<T, VEC, true>, grid, dim3(256), 0, stream, (const T *)x.p, x.ld,
-                             (const T *)residual.p, residual.ld, (T *)y.p, y.ld, rows, cols, key));
-  } else {
-    AB200_CUDA(launchChained(dropoutKernel<T, VEC, false>, grid, dim3(256), 0, stream, (const T *)x.p, x.ld,
-                             (const T *)nullptr, 0LL, (T *)y.p, y.ld, rows, cols, key));
-  }
+  AB200_CUDA(launchChained(dropoutKernel<T, VEC, RES, FLAT>, grid, dim3(256), 0, stream, (const T *)x.p, x.ld,
+                           (const T *)residual.p, residual.ld, (T *)y.p, y.ld, rows, cols, key));
   AB200_LAUNCH_CHECK();
+}
+template <typename T>
+void dropoutOfType(RowsIn x, RowsIn residual, RowsOut y, long long rows, int cols, int type, const DropKey &key,
+                   cudaStream_t stream) {
+  const bool vec = cols % 8 == 0 && spansAlign(x.p, x.ld, type) && spansAlign(y.p, y.ld, type) &&
+                   spansAlign(residual.p, residual.ld, type);
+  if (!vec) {
+    residual.p ? launchDropout<T, false, true, false>(x, residual, y, rows, cols, key, stream)
+               : launchDropout<T, false, false, false>(x, residual, y, rows, cols, key, stream);
+  } else if (rows == 1 || (x.ld == cols && y.ld == cols && (!residual.p || residual.ld == cols) &&
+                           rows * cols <= 0x40000000LL)) {
+    cols = (int)(rows * cols);
+    residual.p ? launchDropout<T, true, true, true>(x, residual, y, 1, cols, key, stream)
+               : launchDropout<T, true, false, true>(x, residual, y, 1, cols, key, stream);
+  } else {
+    residual.p ? launchDropout<T, true, true, false>(x, residual, y, rows, cols, key, stream)
+               : launchDropout<T, true, false, false>(x, residual, y, rows, cols, key, stream);
+  }
 }
 
 } // namespace
 
-void dropoutApply(RowsIn x, RowsIn residual, RowsOut y, long long rows, int cols, int type,
-                  const DropoutArgs &drop, cudaStream_t stream) {
+void dropoutApply(RowsIn x, RowsIn residual, RowsOut y, long long rows, int cols, int type, const DropoutArgs &drop,
+                  cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) {
     return;
   }
   const DropKey key = dropKey(drop);
-  bool vec = cols % 8 == 0 && spansAlign(x.p, x.ld, type) && spansAlign(y.p, y.ld, type) &&
-             spansAlign(residual.p, residual.ld, type);
-  // rows that follow each other without a gap are one row: the blocks of eight are numbered alike
-  if (vec && x.ld == cols && y.ld == cols && (!residual.p || residual.ld == cols) &&
-      rows * cols <= 0x40000000LL) {
-    cols = (int)(rows * cols);
-    rows = 1;
-  }
   switch (type) {
-  case DT_F32:
-    vec ? launchDropout<float, true>(x, residual, y, rows, cols, key, stream)
-        : launchDropout<float, false>(x, residual, y, rows, cols, key, stream);
-    break;
-  case DT_F16:
-    vec ? launchDropout<__half, true>(x, residual, y, rows, cols, key, stream)
-        : launchDropout<__half, false>(x, residual, y, rows, cols, key, stream);
-    break;
-  default:
-    vec ? launchDropout<__nv_bfloat16, true>(x, residual, y, rows, cols, key, stream)
-        : launchDropout<__nv_bfloat16, false>(x, residual, y, rows, cols, key, stream);
+  case DT_F32: dropoutOfType<float>(x, residual, y, rows, cols, type, key, stream); break;
+  case DT_F16: dropoutOfType<__half>(x, residual, y, rows, cols, type, key, stream); break;
+  default: dropoutOfType<__nv_bfloat16>(x, residual, y, rows, cols, type, key, stream);
   }
 }
 

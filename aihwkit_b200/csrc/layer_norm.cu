@@ -138,11 +138,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : kRowThreads)
     for (int s = 0; s < NS; s++) {
       rx[s].get(v[s]);
       if (a.drop) {
-        const uint32_t keep = keepOfSpan<VEC>(key, row, w0 + s * sh.warps_per_row, lane, sh.cols);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          v[s][i] = (keep >> i) & 1u ? v[s][i] * key.scale : 0.0f;
-        }
+        dropSpan(key, keepOfSpan<VEC>(key, row, w0 + s * sh.warps_per_row, lane, sh.cols), v[s]);
       }
       if (a.res) {
         float r[8];
@@ -233,7 +229,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : kRowThreads)
     const float mean = a.mean[row], rstd = a.rstd[row];
     float u[NS][8], t[NS][8];
     Raw8<T, VEC> rx[NS], rr[NS], rg[NS], ra[NS];
-    uint32_t keep[NS];
+    Kept kept[NS];
 #pragma unroll
     for (int s = 0; s < NS; s++) {
       const int span = w0 + s * sh.warps_per_row;
@@ -260,15 +256,11 @@ __global__ void __launch_bounds__(WIDE ? 512 : kRowThreads)
       loadParam<VEC>(a.w, a.w_type, 1.0f, span, lane, sh.cols, w);
       rx[s].get(u[s]);
       rg[s].get(g);
-      keep[s] = 0xffu;
       if (a.drop || a.dx) {
-        keep[s] = keepOfSpan<VEC>(key, row, span, lane, sh.cols);
+        kept[s] = keepOfSpan<VEC>(key, row, span, lane, sh.cols);
       }
       if (a.drop) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          u[s][i] = (keep[s] >> i) & 1u ? u[s][i] * key.scale : 0.0f;
-        }
+        dropSpan(key, kept[s], u[s]);
       }
       if (a.res) {
         float r[8];
@@ -312,10 +304,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : kRowThreads)
         storeSpan<T, VEC>((T *)a.dh + row * a.dh_ld, span, lane, sh.cols, d);
       }
       if (a.dx) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          d[i] = (keep[s] >> i) & 1u ? d[i] * key.scale : 0.0f;
-        }
+        dropSpan(key, kept[s], d);
         storeSpan<T, VEC>((T *)a.dx + row * a.dx_ld, span, lane, sh.cols, d);
       }
     }
