@@ -5,24 +5,26 @@
 // and b are the same sum over rows, u^T x.
 //
 // lowRankApplyKernel. The work is narrow: 2 rank operations per element of x and of y, so memory
-// bounds it up to ranks of about 64. A block takes up to 64 (or 16) rows of one request through both
+// bounds it up to ranks of about 64. A block takes up to 64 (32, 16) rows of one request through both
 // products: x is read once, v stays in shared memory, y is written once; nothing but the saved v
-// goes through memory between the two. Operands go from global memory straight into the fragments
-// of mma.sync: a dot product may run in any order, so a thread takes 16 neighbouring bytes of a row as
-// its share of k, and columns are dealt to the fragments so that a thread ends up with 32
-// neighbouring bytes of y. No operand is used by two warps, so staging would only add traffic. Where rows
+// goes through memory between the two. A dot product may run in any order, so a thread takes 16
+// neighbouring bytes of a row as its share of k, and columns are dealt to the fragments of mma.sync so that it ends up
+// with 16 neighbouring bytes of y. Every warp has its own steps along k and its own columns and
+// fetches them with cp.async into a ring of its own, x and a first, then base and b: loads stay in flight through both
+// products and the sum between them, and no barrier stands in the loops. Where rows
 // are few, a cluster of blocks shares a row tile: each takes a share of k, the partial v are added
 // through distributed shared memory in rank order, and each block takes a share of the columns.
 // Products: bf16 x bf16 and fp16 x fp16 are exact in the fp32 sum; fp32 factors (v, and x, a, b of
 // fp32 calls) are split into two TF32 parts, hi + lo, and multiplied as hi hi + lo hi + hi lo, which leaves
 // 2^-22 of a product out.
 //
-// lowRankGradKernel. grad[id] = sum over the rows of id of u^T x: a warp holds rank x 64 (or 32)
-// columns in fragments and walks a chunk of rows of one request; chunks' partial sums go through memory
-// and are added in the order of the rows (no atomics).
+// lowRankGradKernel. grad[id] = sum over the rows of id of u^T x: a warp holds rank x 128 bytes of columns
+// in fragments and walks a chunk of rows of one request, fetched the same way; chunks' partial sums go
+// through memory and are added in the order of the rows (no atomics).
 #include "digital.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -43,6 +45,8 @@ struct Segments {
 };
 struct RowTile {
   int row0, rows, id; // id < 0: no adapter
+  int seg;            // the request
+  bool alone;         // it has one row
 };
 __device__ __forceinline__ int border(const Segments &s, int j) {
   return j == 0 ? 0 : j == s.n + 2 ? s.rows : min(max(s.starts[j - 1], 0), s.rows);
@@ -53,6 +57,7 @@ __device__ __forceinline__ RowTile findTile(const Segments &s, int slot) {
   if (s.starts == nullptr) {
     t.row0 = slot; // one row each
     t.rows = slot < s.rows ? 1 : 0;
+    t.alone = true;
   } else {
     // the last segment whose first slot is not behind this one; every warp searches, 32 probes at a time
     const int lane = threadIdx.x & 31;
@@ -70,13 +75,57 @@ __device__ __forceinline__ RowTile findTile(const Segments &s, int slot) {
     const long long row0 = begin + ((long long)(slot - (begin >> s.shift) - lo) << s.shift);
     t.rows = row0 < begin ? 0 : (int)max(0LL, min((long long)end - row0, 1LL << s.shift));
     t.row0 = t.rows > 0 ? (int)row0 : 0;
+    t.alone = end == begin + 1;
     seg = lo - 1;
   }
+  t.seg = seg;
   t.id = t.rows > 0 && seg >= 0 && seg < s.n ? s.ids[seg] : -1;
   if (t.id >= s.adapters) {
     t.id = -1;
   }
   return t;
+}
+// Rows of a tile of 16. A request of one row (decoding) shares its tile with the others of one row and the same
+// adapter among its 1024 neighbours, sixteen at a time, so that the adapter is read once for them; the first
+// of the sixteen keeps the tile, for the others this returns false. All warps of all blocks of a tile find the same.
+__device__ __forceinline__ bool gatherRows(const Segments &s, RowTile &tile, int lane, int list[16]) {
+  if (lane < 16) {
+    list[lane] = tile.row0 + min(lane, tile.rows - 1);
+  }
+  if (tile.rows == 1 && tile.id >= 0 && tile.alone) {
+    const int first = tile.seg & ~1023, end = min(first + 1024, s.n);
+    int before = 0, found = 0; // of the adapter's single rows: ahead of this one, all so far
+    for (int w = first; w < end && found - before < 16; w += 32) {
+      const int j = w + lane;
+      bool match = j < end && s.ids[j] == tile.id;
+      int row = j;
+      if (match && s.starts != nullptr) {
+        row = border(s, j + 1);
+        match = border(s, j + 2) == row + 1;
+      }
+      const unsigned hits = __ballot_sync(0xffffffffu, match);
+      if (tile.seg >= w) { // up to this row's own place
+        before += __popc(tile.seg < w + 32 ? hits & ((1u << (tile.seg - w)) - 1u) : hits);
+        if (tile.seg < w + 32 && before % 16 != 0) {
+          return false;
+        }
+      }
+      if (tile.seg < w + 32) {
+        const int at = found + __popc(hits & ((1u << lane) - 1u)) - before;
+        if (match && at >= 0 && at < 16) {
+          list[at] = row;
+        }
+      }
+      found += __popc(hits);
+    }
+    tile.rows = min(found - before, 16);
+    __syncwarp();
+    if (lane >= tile.rows && lane < 16) {
+      list[lane] = list[0];
+    }
+  }
+  __syncwarp();
+  return true;
 }
 long long segmentSlots(const LowRankRows &s, int shift) {
   return s.starts ? (s.rows >> shift) + s.segments + 2 : s.rows;
@@ -84,23 +133,37 @@ long long segmentSlots(const LowRankRows &s, int shift) {
 
 // ---- fragments --------------------------------------------------------------------------------
 __device__ __forceinline__ void mmaTf32(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},"
                "{%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the first product of a sum: c = a b
+__device__ __forceinline__ void mmaTf32First(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// Four 8 x 16-byte matrices, whose rows are at the addresses of lanes 0-7, 8-15, 16-23 and 24-31: lane l gets word l % 4
+// of row l / 4 of each - the operands of mma.sync for 16-bit types and, word by word, for TF32.
+__device__ __forceinline__ void loadMatrices(uint32_t src, uint32_t r[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(src)
+               : "memory");
 }
 template <typename T>
 __device__ __forceinline__ void mma16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16<__nv_bfloat16>(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},"
                "{%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma16<__half>(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},"
                "{%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -147,80 +210,128 @@ template <typename T> __device__ __forceinline__ float elemOf(const uint4 &q, in
     return (i & 1) ? f.y : f.x;
   }
 }
-__device__ __forceinline__ uint32_t wordOf(const uint4 &q, int i) {
-  return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w;
-}
 
-// c += a b for one k-share of 16 bytes a row: x rows g and g + 8, factor row g
-template <typename T>
-__device__ __forceinline__ void mmaShare(float c[4], const uint4 &xg, const uint4 &xg8, const uint4 &f) {
-  if constexpr (sizeof(T) == 4) {
+// acc[i][j] += x_i f_j for a step of 64 bytes along k, whose halves h have the operands x[i][h][0..3] and
+// f[j][2 h], f[j][2 h + 1]. Each term goes through all fragments before the next: products into one sum
+// wait for each other.
+template <typename T, int MT, int NT>
+__device__ __forceinline__ void mmaStep(float (&acc)[MT][NT][4], uint32_t (&x)[MT][2][4], const uint32_t (&f)[NT][4]) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      uint32_t ah[4], al[4], bh[2], bl[2];
-      split(__uint_as_float(wordOf(xg, 2 * h)), ah[0], al[0]);
-      split(__uint_as_float(wordOf(xg8, 2 * h)), ah[1], al[1]);
-      split(__uint_as_float(wordOf(xg, 2 * h + 1)), ah[2], al[2]);
-      split(__uint_as_float(wordOf(xg8, 2 * h + 1)), ah[3], al[3]);
-      split(__uint_as_float(wordOf(f, 2 * h)), bh[0], bl[0]);
-      split(__uint_as_float(wordOf(f, 2 * h + 1)), bh[1], bl[1]);
-      mmaTf32(c, al, bh[0], bh[1]);
-      mmaTf32(c, ah, bl[0], bl[1]);
-      mmaTf32(c, ah, bh[0], bh[1]);
-    }
-  } else {
+  for (int h = 0; h < 2; h++) {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t xl[MT][4], fh[NT][2], fl[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t a[4] = {wordOf(xg, 2 * h), wordOf(xg8, 2 * h), wordOf(xg, 2 * h + 1), wordOf(xg8, 2 * h + 1)};
-      mma16<T>(c, a, wordOf(f, 2 * h), wordOf(f, 2 * h + 1));
+      for (int i = 0; i < MT; i++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          split(__uint_as_float(x[i][h][e]), x[i][h][e], xl[i][e]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        split(__uint_as_float(f[j][2 * h]), fh[j][0], fl[j][0]);
+        split(__uint_as_float(f[j][2 * h + 1]), fh[j][1], fl[j][1]);
+      }
+#pragma unroll
+      for (int term = 0; term < 3; term++) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+#pragma unroll
+          for (int i = 0; i < MT; i++) {
+            mmaTf32(acc[i][j], term == 0 ? xl[i] : x[i][h], term == 1 ? fl[j][0] : fh[j][0], term == 1 ? fl[j][1] : fh[j][1]);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          mma16<T>(acc[i][j], x[i][h], f[j][2 * h], f[j][2 * h + 1]);
+        }
+      }
     }
   }
 }
-// c[j] += (hi + lo) b for the neighbouring columns j of one thread: b0 from row t of the factor, b1
-// from row t + 4
-template <typename T, int NJ>
-__device__ __forceinline__ void mmaColumns(float (*c)[4], const uint32_t hi[4], const uint32_t lo[4], const uint4 &b0,
-                                           const uint4 &b1) {
+// acc[i][j] += (hi_i + lo_i) b_j for the neighbouring columns j of one thread: b0 from row t of the
+// factor, b1 from row t + 4. FIRST: acc is set, not added to
+template <typename T, bool FIRST, int MT, int NJ>
+__device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], const uint32_t (&hi)[MT][4], const uint32_t (&lo)[MT][4],
+                                           const uint4 &b0, const uint4 &b1) {
+  uint32_t b[NJ][2], bl[NJ][2];
 #pragma unroll
   for (int j = 0; j < NJ; j++) {
     const float f0 = elemOf<T>(b0, j), f1 = elemOf<T>(b1, j);
     if constexpr (sizeof(T) == 4) {
-      uint32_t h0, l0, h1, l1;
-      split(f0, h0, l0);
-      split(f1, h1, l1);
-      mmaTf32(c[j], lo, h0, h1);
-      mmaTf32(c[j], hi, l0, l1);
-      mmaTf32(c[j], hi, h0, h1);
+      split(f0, b[j][0], bl[j][0]);
+      split(f1, b[j][1], bl[j][1]);
     } else {
-      mmaTf32(c[j], lo, __float_as_uint(f0), __float_as_uint(f1));
-      mmaTf32(c[j], hi, __float_as_uint(f0), __float_as_uint(f1));
+      b[j][0] = __float_as_uint(f0);
+      b[j][1] = __float_as_uint(f1);
+    }
+  }
+#pragma unroll
+  for (int term = 0; term < 3; term++) {
+    if (term == 1 && sizeof(T) != 4) {
+      continue; // 16-bit factors have no lower part
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        if (FIRST && term == 0) {
+          mmaTf32First(acc[i][j], lo[i], b[j][0], b[j][1]);
+        } else {
+          mmaTf32(acc[i][j], term == 0 ? lo[i] : hi[i], term == 1 ? bl[j][0] : b[j][0], term == 1 ? bl[j][1] : b[j][1]);
+        }
+      }
     }
   }
 }
 
-// 32 neighbouring bytes of a row: 16 16-bit or eight fp32 elements
+// ---- rings of cp.async ------------------------------------------------------------------------
+// 16 bytes of a row to shared memory, from `src`, the place of column `col`; columns past the end, and all
+// of them where `in` is false, become zeros without a read (nor a branch). Rows that 16-byte
+// accesses do not fit go by elements: fp32 still asynchronously, 16-bit ones through registers.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load32Bytes(const T *row, int col, int cols, uint4 q[2]) {
-  q[0] = load16B<T, VEC>(row, col, cols);
-  q[1] = load16B<T, VEC>(row, col + 16 / (int)sizeof(T), cols);
+__device__ __forceinline__ void fetch16B(uint32_t dst, const T *src, int col, int cols, bool in) {
+  if (VEC) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in && col < cols ? 16 : 0)
+                 : "memory");
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * i), "l"(src + i),
+                   "r"(in && col + i < cols ? 4 : 0)
+                   : "memory");
+    }
+  } else {
+    const uint4 q = load16B<T, false>(src - col, col, in ? cols : 0);
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+  }
+}
+__device__ __forceinline__ void fetchCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the newest N groups of this thread have arrived
+template <int N> __device__ __forceinline__ void fetchWait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 shared16B(const unsigned char *src) { return *reinterpret_cast<const uint4 *>(src); }
+__device__ __forceinline__ uint4 shared8B(const unsigned char *src) {
+  const uint2 q = *reinterpret_cast<const uint2 *>(src);
+  return make_uint4(q.x, q.y, 0, 0);
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store32Bytes(T *row, int col, int cols, const float *v) {
-  constexpr int E = 32 / sizeof(T);
+__device__ __forceinline__ void store16B(T *row, int col, int cols, const float *v) {
+  constexpr int E = 16 / sizeof(T);
   if (VEC) {
     if (col < cols) {
       if constexpr (sizeof(T) == 4) {
-        store32B(reinterpret_cast<float *>(row) + col, v);
+        *reinterpret_cast<float4 *>(row + col) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          uint4 q;
-          q.x = pack2<T>(v[8 * h], v[8 * h + 1]);
-          q.y = pack2<T>(v[8 * h + 2], v[8 * h + 3]);
-          q.z = pack2<T>(v[8 * h + 4], v[8 * h + 5]);
-          q.w = pack2<T>(v[8 * h + 6], v[8 * h + 7]);
-          reinterpret_cast<uint4 *>(row + col)[h] = q;
-        }
+        uint4 q;
+        q.x = pack2<T>(v[0], v[1]);
+        q.y = pack2<T>(v[2], v[3]);
+        q.z = pack2<T>(v[4 % E], v[5 % E]);
+        q.w = pack2<T>(v[6 % E], v[7 % E]);
+        *reinterpret_cast<uint4 *>(row + col) = q;
       }
     }
   } else {
@@ -245,74 +356,136 @@ struct Apply {
   int cluster;
 };
 
-constexpr int kApplyThreads = 256;
+// MT fragments of 16 rows; ranks go through the products 8 * NT at a time. A stage of a warp's ring has 64
+// bytes of each row of x (base) and of 8 * NT rows of a (b). Tiles of 16 rows have eight warps, as
+// their time is that of a chain of loads and sums, and the others four.
+template <int MT, int NT> struct ApplyShape {
+  static constexpr int TM = 16 * MT, RC = 8 * NT, W = MT == 1 ? 8 : 4;
+  static constexpr int XB = TM * 64, STAGE = XB + RC * 64;
+  static constexpr int STAGES = MT == 4 || NT == 8 ? 2 : MT == 2 || NT == 4 ? 3 : 4;
+  static constexpr int RING = W * STAGES * STAGE;
+  // shares of the warps of a tile of 16 rows, added after one barrier; larger tiles add them in turn
+  static constexpr int SHARES = MT == 1 ? W * TM * (RC + 4) * 4 : 0;
+  // blocks to a multiprocessor, bounded by registers and shared memory
+  static constexpr int BLOCKS = MT == 1 ? 2 : 4;
+  static size_t bytes(int rank) {
+    const int vs = ((rank + 7) & ~7) + 4;
+    return RING + SHARES + (size_t)TM * ((vs - 4) * 8 + vs * 4);
+  }
+};
 
-// MT fragments of 16 rows per warp, WM warps over the rows, the other warps share k and the columns;
-// ranks go through the first product 8 * NT at a time
-template <typename T, bool VEC, int MT, int WM, int NT>
-__global__ void __launch_bounds__(kApplyThreads, 2) lowRankApplyKernel(Apply p) {
-  constexpr int WARPS = kApplyThreads / 32, WK = WARPS / WM, TM = 16 * MT * WM, RC = 8 * NT, RS = RC + 4;
-  constexpr int E = 16 / sizeof(T), KS = 4 * E; // elements of k per thread, per fragment row and step
-  constexpr int NJ = E, UC = 8 * NJ;            // columns per thread of a factor, per unit of a warp
-  extern __shared__ float smem[];
+template <typename T, bool VEC, int MT, int NT>
+__global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT>::BLOCKS)) lowRankApplyKernel(Apply p) {
+  using Shape = ApplyShape<MT, NT>;
+  constexpr int W = Shape::W, TM = Shape::TM, RC = Shape::RC, S = Shape::STAGES;
+  constexpr int E = 16 / sizeof(T), KS = 4 * E; // elements in 16 bytes, of k in a step, of columns in a unit
+  constexpr int NJ = E / 2;                     // fragments beside each other in a unit
+  extern __shared__ __align__(16) unsigned char smem[];
   pdlEnter();
   const int part = p.cluster > 1 ? blockIdx.x % p.cluster : 0;
-  const RowTile tile = findTile(p.seg, blockIdx.x / p.cluster);
+  RowTile tile = findTile(p.seg, blockIdx.x / p.cluster);
   if (tile.rows <= 0) {
     return; // the whole cluster has the same tile
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int wm = warp / WK, wk = warp % WK;
-  const int units = (p.n + UC - 1) / UC, units_per = (units + p.cluster - 1) / p.cluster;
-  const int u_begin = part * units_per, u_end = min(units, u_begin + units_per);
-  int row[MT][2]; // rows of this thread's fragments, -1 past the tile
-#pragma unroll
-  for (int i = 0; i < MT; i++) {
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int r = wm * 16 * MT + i * 16 + h * 8 + g;
-      row[i][h] = r < tile.rows ? tile.row0 + r : -1;
+  __shared__ int tile_rows[MT == 1 ? W : 1][16]; // rows of a tile of 16, a copy for each warp
+  if (MT == 1) {
+    if (!gatherRows(p.seg, tile, lane, tile_rows[warp])) {
+      return; // another tile has this row
     }
   }
+  const int units = (p.n + KS - 1) / KS, units_per = (units + p.cluster - 1) / p.cluster;
+  const int u_begin_all = min(units, part * units_per), u_end = min(units, part * units_per + units_per);
+  const int u_begin = u_begin_all + warp;
+  const T *x = (const T *)p.x + tile.row0 * p.x_ld;
+  const T *base = (const T *)p.base + tile.row0 * p.base_ld;
+  T *y = (T *)p.y + tile.row0 * p.y_ld;
+  // rows g and g + 8 of a tile of 16 against row0, and the distance between them; in a larger one they
+  // follow each other
+  const long long row_g = MT == 1 ? tile_rows[warp][g] - tile.row0 : g;
+  const long long row_8 = MT == 1 ? tile_rows[warp][g + 8] - tile_rows[warp][g] : 8;
   if (tile.id < 0) {
     // no adapter: y is base (nothing to do where they are the same memory) or zero
     if (p.y == nullptr || p.y == p.base) {
       return;
     }
-    for (int u = u_begin + wk; u < u_end; u += WK) {
-      const int col = u * UC + 2 * NJ * t;
+    // eight rows of a warp's 512 bytes at a time, all read before the first is written: a block's copy is a
+    // chain of such turns, and with fewer rows to a turn it outlasted the tiles that compute
+    const int chunks = (u_end - u_begin_all + 7) / 8; // of 512 bytes
+    for (int i = warp; i < chunks * ((tile.rows + 7) / 8); i += W) {
+      const int col = (u_begin_all + i % chunks * 8) * KS + lane * E, r = i / chunks * 8;
+      const bool in = col < u_end * KS;
+      uint4 q[8];
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
+      for (int j = 0; j < 8; j++) {
+        q[j] = p.base && in && r + j < tile.rows ? load16B<T, VEC>(base + (r + j) * p.base_ld, col, p.n) : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          if (row[i][h] >= 0) {
-            uint4 q[2] = {};
-            if (p.base) {
-              load32Bytes<T, VEC>((const T *)p.base + row[i][h] * p.base_ld, col, p.n, q);
-            }
-            float o[2 * NJ];
+      for (int j = 0; j < 8; j++) {
+        float o[E];
 #pragma unroll
-            for (int j = 0; j < 2 * NJ; j++) {
-              o[j] = elemOf<T>(q[j / NJ], j % NJ);
-            }
-            store32Bytes<T, VEC>((T *)p.y + row[i][h] * p.y_ld, col, p.n, o);
-          }
+        for (int e = 0; e < E; e++) {
+          o[e] = elemOf<T>(q[j], e);
+        }
+        if (in && r + j < tile.rows) {
+          store16B<T, VEC>(y + (r + j) * p.y_ld, col, p.n, o);
         }
       }
     }
     return;
   }
   const int r_pad = (p.rank + 7) & ~7, vs = r_pad + 4;
-  float *mine = smem;             // [TM][vs]: this block's share of v
-  float *red = smem + TM * vs;    // [WK][TM][RS] while the warps' shares are added
-  float *full = p.cluster > 1 ? red : mine; // [TM][vs]: v of the tile
+  const unsigned char *held = smem + warp * S * Shape::STAGE; // this warp's ring, as it is read
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(held);
+  // v of the tile as the second product's operands: [fragment][8 ranks][hi, lo][lane][4]
+  float *v = reinterpret_cast<float *>(smem + Shape::RING);
+  float *mine = v + TM * r_pad * 2; // [TM][vs]: this block's share of v
+  float *shares = mine + TM * vs;   // [W][TM][RC + 4], of tiles of 16 rows
   const float scale = p.scale[tile.id];
   const T *fa = (const T *)p.a + (long long)tile.id * p.rank * p.k;
   const T *fb = (const T *)p.b + (long long)tile.id * p.rank * p.n;
 
+  // Addresses are kept as one pointer per operand and advanced: with a product per row and access
+  // they were half of all instructions.
+  const int rows_in = tile.rows; // rows q * 8 + g below it are there; others are neither fetched nor stored
+  const T *x_at = x + row_g * p.x_ld + t * E, *base_at = base + row_g * p.base_ld + t * E;
+  T *y_at = y + row_g * p.y_ld + t * E;
+  const long long x_8 = row_8 * p.x_ld, base_8 = row_8 * p.base_ld, y_8 = row_8 * p.y_ld;
+  const uint32_t own = g * 64 + t * 16; // this thread's 16 bytes of the rows g of a stage
+  // While x and a go through, the four 16-byte pieces of a row change places with the row, so that the eight
+  // rows of a matrix lie in different banks
+  const uint32_t own_x = g * 64 + (t ^ ((g >> 1) & 3)) * 16;
+  // matrices of x (rows 0-7 and 8-15 of a fragment, two pieces) and of a (eight rows, four pieces)
+  const uint32_t mat_row = lane & 15, mat_x = mat_row * 64, mat_swz = (mat_row >> 1) & 3, mat_f = (lane & 7) * 64;
+
   // v = x a^T: steps of KS along k are dealt to the blocks of the cluster and to the warps in turn
   const int steps = (p.k + KS - 1) / KS, steps_per = (steps + p.cluster - 1) / p.cluster;
-  const int s_end = min(steps, (part + 1) * steps_per);
+  const int s_begin = part * steps_per + warp, s_end = min(steps, part * steps_per + steps_per);
+  // y = base + v b: units of KS columns, and for each RC ranks at a time; base comes with the last ranks
+  int f_unit = p.y != nullptr ? u_begin : units, f_rank = 0, f_stage = 0; // what fetchUnit takes next
+  const auto fetchUnit = [&]() {
+    if (f_unit < u_end) {
+      const int c0 = f_unit * KS, col = c0 + t * E;
+      const uint32_t dst = ring + f_stage * Shape::STAGE + own;
+      const bool last = f_rank + RC >= p.rank;
+      if (p.base != nullptr && last) {
+        const T *src = base_at + c0;
+#pragma unroll
+        for (int q = 0; q < 2 * MT; q++, src += base_8) {
+          fetch16B<T, VEC>(dst + q * 512, src, col, p.n, q * 8 + g < rows_in);
+        }
+      }
+      const T *src = fb + (long long)(f_rank + g) * p.n + col;
+#pragma unroll
+      for (int j = 0; j < NT; j++, src += 8 * p.n) {
+        fetch16B<T, VEC>(dst + Shape::XB + j * 512, src, col, p.n, f_rank + j * 8 + g < p.rank);
+      }
+      f_rank = last ? 0 : f_rank + RC;
+      f_unit += last ? W : 0;
+    }
+    f_stage = f_stage + 1 == S ? 0 : f_stage + 1;
+    fetchCommit();
+  };
   for (int r0 = 0; r0 < p.rank; r0 += RC) {
     float acc[MT][NT][4];
 #pragma unroll
@@ -322,147 +495,235 @@ __global__ void __launch_bounds__(kApplyThreads, 2) lowRankApplyKernel(Apply p) 
         acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
       }
     }
-#pragma unroll 2
-    for (int s = part * steps_per + wk; s < s_end; s += WK) {
-      const int k0 = s * KS + t * E;
-      uint4 x[MT][2], f[NT];
+    const auto fetchStep = [&](int s, int stage) {
+      if (s < s_end) {
+        const int c0 = s * KS, k0 = c0 + t * E;
+        const uint32_t dst = ring + stage * Shape::STAGE + own_x;
+        const T *src = x_at + c0;
+#pragma unroll
+        for (int q = 0; q < 2 * MT; q++, src += x_8) {
+          fetch16B<T, VEC>(dst + q * 512, src, k0, p.k, q * 8 + g < rows_in);
+        }
+        const T *f = fa + (long long)(r0 + g) * p.k + k0;
+#pragma unroll
+        for (int j = 0; j < NT; j++, f += 8 * p.k) {
+          fetch16B<T, VEC>(dst + Shape::XB + j * 512, f, k0, p.k, r0 + j * 8 + g < p.rank);
+        }
+      }
+      fetchCommit();
+    };
+#pragma unroll
+    for (int q = 0; q < S - 1; q++) {
+      fetchStep(s_begin + q * W, q);
+    }
+    int stage = 0;
+    for (int s = s_begin; s < s_end; s += W) {
+      __syncwarp(); // all lanes have read the stage that is filled now
+      fetchStep(s + (S - 1) * W, stage == 0 ? S - 1 : stage - 1);
+      fetchWait<S - 1>();
+      __syncwarp(); // and see what the others fetched
+      const uint32_t src = ring + stage * Shape::STAGE;
+      uint32_t xf[MT][2][4], f[NT][4];
 #pragma unroll
       for (int i = 0; i < MT; i++) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          x[i][h] = row[i][h] >= 0 ? load16B<T, VEC>((const T *)p.x + row[i][h] * p.x_ld, k0, p.k)
-                                   : make_uint4(0, 0, 0, 0);
+          loadMatrices(src + i * 1024 + mat_x + (((2 * h + (lane >> 4)) ^ mat_swz) * 16), xf[i][h]);
         }
       }
 #pragma unroll
       for (int j = 0; j < NT; j++) {
-        const int r = r0 + j * 8 + g;
-        f[j] = r < p.rank ? load16B<T, VEC>(fa + (long long)r * p.k, k0, p.k) : make_uint4(0, 0, 0, 0);
+        loadMatrices(src + Shape::XB + j * 512 + mat_f + (((lane >> 3) ^ ((lane >> 1) & 3)) * 16), f[j]);
       }
+      mmaStep<T>(acc, xf, f);
+      stage = stage + 1 == S ? 0 : stage + 1;
+    }
+    __syncwarp();
+    if (r0 + RC >= p.rank) {
+      // the ring is read: the first units arrive while the shares of v are added
+#pragma unroll
+      for (int q = 0; q < S - 1; q++) {
+        fetchUnit();
+      }
+    }
+    if (MT == 1) {
 #pragma unroll
       for (int j = 0; j < NT; j++) {
+        float *d = shares + (warp * TM + g) * (RC + 4) + j * 8 + 2 * t;
+        *reinterpret_cast<float2 *>(d) = make_float2(acc[0][j][0], acc[0][j][1]);
+        *reinterpret_cast<float2 *>(d + 8 * (RC + 4)) = make_float2(acc[0][j][2], acc[0][j][3]);
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < TM * RC; e += W * 32) {
+        const int r = e / RC, c = e % RC;
+        if (r0 + c < r_pad) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int w = 0; w < W; w++) {
+            sum += shares[(w * TM + r) * (RC + 4) + c];
+          }
+          mine[r * vs + r0 + c] = sum;
+        }
+      }
+      __syncthreads();
+      continue;
+    }
+    // the warps add their shares one after the other
+    for (int w = 0; w < W; w++) {
+      if (warp == w) {
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-          mmaShare<T>(acc[i][j], x[i][0], x[i][1], f[j]);
+#pragma unroll
+          for (int j = 0; j < NT; j++) {
+            if (r0 + j * 8 < r_pad) {
+              float2 *d = reinterpret_cast<float2 *>(mine + (i * 16 + g) * vs + r0 + j * 8 + 2 * t);
+              float2 *d8 = reinterpret_cast<float2 *>(mine + (i * 16 + g + 8) * vs + r0 + j * 8 + 2 * t);
+              float2 c = make_float2(acc[i][j][0], acc[i][j][1]), c8 = make_float2(acc[i][j][2], acc[i][j][3]);
+              if (w > 0) {
+                const float2 o = *d, o8 = *d8;
+                c.x += o.x;
+                c.y += o.y;
+                c8.x += o8.x;
+                c8.y += o8.y;
+              }
+              *d = c;
+              *d8 = c8;
+            }
+          }
         }
       }
+      __syncthreads();
     }
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (p.cluster > 1) {
+    cluster.sync();
+  }
+  for (int r = threadIdx.x / 8; r < TM; r += W * 4) {
+    for (int c = threadIdx.x % 8; c < r_pad; c += 8) {
+      float sum = 0.0f;
+      if (p.cluster > 1) {
+        float share[8]; // all on their way before the first is added
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-#pragma unroll
-      for (int j = 0; j < NT; j++) {
-        float *d = red + (wk * TM + wm * 16 * MT + i * 16 + g) * RS + j * 8 + 2 * t;
-        *reinterpret_cast<float2 *>(d) = make_float2(acc[i][j][0], acc[i][j][1]);
-        *reinterpret_cast<float2 *>(d + 8 * RS) = make_float2(acc[i][j][2], acc[i][j][3]);
-      }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < TM * RC; e += kApplyThreads) {
-      const int r = e / RC, c = e % RC;
-      if (r0 + c < r_pad) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WK; w++) {
-          sum += red[(w * TM + r) * RS + c];
+        for (int q = 0; q < 8; q++) {
+          share[q] = q < p.cluster ? cluster.map_shared_rank(mine, q)[r * vs + c] : 0.0f;
         }
-        mine[r * vs + r0 + c] = p.cluster > 1 ? sum : sum * scale;
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+          sum += share[q];
+        }
+      } else {
+        sum = mine[r * vs + c];
+      }
+      sum *= scale;
+      uint32_t hi, lo;
+      split(sum, hi, lo);
+      float *d = v + ((r / 16 * (r_pad / 8) + c / 8) * 64 + r % 8 * 4 + c % 4) * 4 + (r % 16) / 8 + (c % 8) / 4 * 2;
+      d[0] = __uint_as_float(hi);
+      d[128] = __uint_as_float(lo);
+      if (p.v != nullptr && part == 0 && r < tile.rows && c < p.rank) {
+        const long long row = MT == 1 ? tile_rows[warp][r] : tile.row0 + r;
+        p.v[row * p.rank + c] = sum;
       }
     }
-    __syncthreads();
   }
   if (p.cluster > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    for (int e = threadIdx.x; e < TM * r_pad; e += kApplyThreads) {
-      const int o = (e / r_pad) * vs + e % r_pad;
-      float sum = 0.0f;
-      for (int q = 0; q < p.cluster; q++) {
-        sum += cluster.map_shared_rank(mine, q)[o];
-      }
-      full[o] = sum * scale;
-    }
-    cluster.sync(); // no block leaves, and none reads `full`, before all have read the shares
-  }
-  if (p.v != nullptr && part == 0) {
-    for (int e = threadIdx.x; e < tile.rows * p.rank; e += kApplyThreads) {
-      p.v[(long long)tile.row0 * p.rank + e] = full[(e / p.rank) * vs + e % p.rank];
-    }
+    cluster.sync(); // no block leaves before all have read its share
+  } else {
+    __syncthreads();
   }
   if (p.y == nullptr) {
     return;
   }
-
-  // y = base + v b: units of UC columns are dealt to the blocks of the cluster and to the warps
-  const float *vrow = full + (wm * 16 * MT + g) * vs + t;
-  for (int u = u_begin + wk; u < u_end; u += WK) {
-    const int col = u * UC + 2 * NJ * t;
-    uint4 old[MT][2][2] = {};
-    if (p.base) {
+  if (p.base == nullptr) { // zeros in its place, in every stage (each thread reads its own)
+    for (int q = 0; q < S * 2 * MT; q++) {
+      *reinterpret_cast<uint4 *>(smem + warp * S * Shape::STAGE + q / (2 * MT) * Shape::STAGE + own + q % (2 * MT) * 512) =
+          make_uint4(0, 0, 0, 0);
+    }
+  }
+  float acc[MT][NJ][4];
+  const uint4 *operands = reinterpret_cast<const uint4 *>(v) + lane;
+  int stage = 0, r0 = 0;
+  for (int u = u_begin; u < u_end;) {
+    __syncwarp(); // all lanes have read the stage that is filled now
+    fetchUnit();
+    fetchWait<S - 1>();
+    __syncwarp(); // b is read by other lanes than fetched it
+    const unsigned char *src = held + stage * Shape::STAGE;
+    stage = stage + 1 == S ? 0 : stage + 1;
+    const auto ranks8 = [&](int r, auto first) {
+      const uint4 b0 = shared8B(src + Shape::XB + (r + t) * 64 + g * 8);
+      const uint4 b1 = shared8B(src + Shape::XB + (r + t + 4) * 64 + g * 8);
+      uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
+      for (int m = 0; m < MT; m++) {
+        const uint4 *q = operands + (m * (r_pad / 8) + (r0 + r) / 8) * 64;
+        const uint4 qh = q[0], ql = q[32];
+        hi[m][0] = qh.x, hi[m][1] = qh.y, hi[m][2] = qh.z, hi[m][3] = qh.w;
+        lo[m][0] = ql.x, lo[m][1] = ql.y, lo[m][2] = ql.z, lo[m][3] = ql.w;
+      }
+      mmaColumns<T, decltype(first)::value>(acc, hi, lo, b0, b1);
+    };
+    if (r0 == 0) {
+      ranks8(0, std::true_type());
+    } else {
+      ranks8(0, std::false_type());
+    }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          if (row[i][h] >= 0) {
-            load32Bytes<T, VEC>((const T *)p.base + row[i][h] * p.base_ld, col, p.n, old[i][h]);
+    for (int r = 8; r < RC; r += 8) {
+      if (r0 + r < r_pad) {
+        ranks8(r, std::false_type());
+      }
+    }
+    if (r0 + RC < p.rank) {
+      r0 += RC;
+      continue;
+    }
+    const int col = u * KS + t * E;
+    T *dst = y_at + u * KS;
+#pragma unroll
+    for (int q = 0; q < 2 * MT; q++, dst += y_8) {
+      if (q * 8 + g < rows_in) {
+        const uint4 old = shared16B(src + own + q * 512);
+        float o[E];
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+          o[j] = acc[q / 2][j][2 * (q % 2)] + elemOf<T>(old, j);
+          o[NJ + j] = acc[q / 2][j][2 * (q % 2) + 1] + elemOf<T>(old, NJ + j);
+        }
+        if (VEC) {
+          if (col < p.n) {
+            store16B<T, true>(dst, 0, E, o);
           }
+        } else {
+          store16B<T, false>(dst - col, col, p.n, o);
         }
       }
     }
-    float acc[MT][NJ][4];
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-#pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
-      }
-    }
-    const int fcol = u * UC + NJ * g;
-#pragma unroll 2
-    for (int r = 0; r < r_pad; r += 8) {
-      const uint4 none = make_uint4(0, 0, 0, 0);
-      const uint4 b0 = r + t < p.rank ? load16B<T, VEC>(fb + (long long)(r + t) * p.n, fcol, p.n) : none;
-      const uint4 b1 = r + t + 4 < p.rank ? load16B<T, VEC>(fb + (long long)(r + t + 4) * p.n, fcol, p.n) : none;
-#pragma unroll
-      for (int i = 0; i < MT; i++) {
-        uint32_t hi[4], lo[4];
-        const float *v = vrow + i * 16 * vs + r;
-        split(v[0], hi[0], lo[0]);
-        split(v[8 * vs], hi[1], lo[1]);
-        split(v[4], hi[2], lo[2]);
-        split(v[8 * vs + 4], hi[3], lo[3]);
-        mmaColumns<T, NJ>(acc[i], hi, lo, b0, b1);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if (row[i][h] >= 0) {
-          float o[2 * NJ];
-#pragma unroll
-          for (int j = 0; j < NJ; j++) {
-            o[j] = acc[i][j][2 * h] + elemOf<T>(old[i][h][0], j);
-            o[NJ + j] = acc[i][j][2 * h + 1] + elemOf<T>(old[i][h][1], j);
-          }
-          store32Bytes<T, VEC>((T *)p.y + row[i][h] * p.y_ld, col, p.n, o);
-        }
-      }
-    }
+    r0 = 0;
+    u += W;
   }
 }
 
-template <typename T, bool VEC, int MT, int WM, int NT>
-void launchApply(Apply p, long long slots, cudaStream_t stream) {
-  constexpr int WK = kApplyThreads / 32 / WM, TM = 16 * MT * WM;
-  const int vs = ((p.rank + 7) & ~7) + 4;
-  const size_t smem = sizeof(float) * ((size_t)TM * vs + std::max((size_t)WK * TM * (8 * NT + 4), (size_t)TM * vs));
-  auto kernel = lowRankApplyKernel<T, VEC, MT, WM, NT>;
+template <typename T, bool VEC, int MT, int NT>
+void launchApply(Apply p, const LowRankRows &seg, int shift, cudaStream_t stream) {
+  p.seg.shift = shift;
+  const long long slots = segmentSlots(seg, shift);
+  // Blocks that share a tile: as many as fit the GPU at once, eight at most. Of tiles of one row, those
+  // that find others of their adapter make one; of 256 rows with 64 adapters about 80 stay.
+  const long long active = MT == 1 ? std::min(slots, p.seg.adapters + slots / 16) : slots;
+  p.cluster = 1;
+  while (p.cluster < 8 && active * p.cluster * 2 <= (long long)ApplyShape<MT, NT>::BLOCKS * digitalSmCount()) {
+    p.cluster *= 2;
+  }
+  const size_t smem = ApplyShape<MT, NT>::bytes(p.rank);
+  auto kernel = lowRankApplyKernel<T, VEC, MT, NT>;
   if (smem > 48 * 1024) {
     AB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(slots * p.cluster));
-  cfg.blockDim = dim3(kApplyThreads);
+  cfg.blockDim = dim3(ApplyShape<MT, NT>::W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -476,32 +737,28 @@ void launchApply(Apply p, long long slots, cudaStream_t stream) {
   AB200_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
   AB200_LAUNCH_CHECK();
 }
-template <typename T, bool VEC, int MT, int WM> void dispatchRank(const Apply &p, long long slots, cudaStream_t st) {
-  if (p.rank <= 8) {
-    launchApply<T, VEC, MT, WM, 1>(p, slots, st);
+template <typename T, bool VEC> void dispatchApply(const Apply &p, const LowRankRows &seg, cudaStream_t st) {
+  // Requests of 16 rows and fewer on average (decoding) take tiles of 16 rows, longer ones of 64, or 32 with
+  // more than 16 ranks: with the fragments of 64 rows only three blocks fitted a multiprocessor (8192 rows,
+  // 4096 -> 4096, rank 32, bf16: 78 us, 65 with 32 rows and one stage more)
+  if (seg.starts == nullptr || seg.rows <= 16LL * seg.segments) {
+    if (p.rank <= 8) {
+      launchApply<T, VEC, 1, 1>(p, seg, 4, st);
+    } else if (p.rank <= 16) {
+      launchApply<T, VEC, 1, 2>(p, seg, 4, st);
+    } else if (p.rank <= 32) {
+      launchApply<T, VEC, 1, 4>(p, seg, 4, st);
+    } else {
+      launchApply<T, VEC, 1, 8>(p, seg, 4, st);
+    }
+  } else if (p.rank <= 8) {
+    launchApply<T, VEC, 4, 1>(p, seg, 6, st);
   } else if (p.rank <= 16) {
-    launchApply<T, VEC, MT, WM, 2>(p, slots, st);
+    launchApply<T, VEC, 4, 2>(p, seg, 6, st);
   } else if (p.rank <= 32) {
-    launchApply<T, VEC, MT, WM, 4>(p, slots, st);
+    launchApply<T, VEC, 2, 4>(p, seg, 5, st);
   } else {
-    launchApply<T, VEC, MT, WM, 8>(p, slots, st);
-  }
-}
-template <typename T> void dispatchApply(Apply p, const LowRankRows &seg, bool vec, cudaStream_t st) {
-  // Requests of 16 rows and fewer on average (decoding) take tiles of 16 rows, longer ones of 64.
-  const bool small = seg.starts == nullptr || seg.rows <= 16LL * seg.segments;
-  p.seg.shift = small ? 4 : 6;
-  const long long slots = segmentSlots(seg, p.seg.shift);
-  // Blocks that share a tile: as many as it takes to occupy the multiprocessors, eight at most
-  const int sms = digitalSmCount();
-  p.cluster = 1;
-  while (p.cluster < 8 && slots * p.cluster < sms) {
-    p.cluster *= 2;
-  }
-  if (small) {
-    vec ? dispatchRank<T, true, 1, 1>(p, slots, st) : dispatchRank<T, false, 1, 1>(p, slots, st);
-  } else {
-    vec ? dispatchRank<T, true, 2, 2>(p, slots, st) : dispatchRank<T, false, 2, 2>(p, slots, st);
+    launchApply<T, VEC, 2, 8>(p, seg, 5, st);
   }
 }
 
@@ -517,11 +774,21 @@ struct Grad {
   int rank, rank_passes;
 };
 
-constexpr int kGradWarps = 4;
+constexpr int kGradWarps = 4, kGradRows = 32, kGradStages = 3;
+
+// a stage: 32 rows of 128 bytes for every warp, and the ranks of the same rows of u for all of them (rows of
+// 16 RT + 8 floats: the eight ranks x four rows of a fragment then lie in different banks)
+template <int RT> struct GradShape {
+  static constexpr int US = 16 * RT + 8;
+  static constexpr int XB = kGradRows * 128, STAGE = kGradWarps * XB + kGradRows * US * 4;
+  static constexpr int BYTES = kGradStages * STAGE;
+};
 
 template <typename T, bool VEC, int RT>
-__global__ void __launch_bounds__(kGradWarps * 32) lowRankGradKernel(Grad p) {
-  constexpr int NJ = 16 / sizeof(T), UC = 8 * NJ;
+__global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradKernel(Grad p) {
+  using Shape = GradShape<RT>;
+  constexpr int E = 16 / sizeof(T), NJ = E, UC = 8 * NJ, S = kGradStages;
+  extern __shared__ __align__(16) unsigned char smem[];
   pdlEnter();
   const int side = blockIdx.z / p.rank_passes, r0 = (blockIdx.z % p.rank_passes) * 16 * RT;
   const RowTile tile = findTile(p.seg, blockIdx.x);
@@ -531,14 +798,38 @@ __global__ void __launch_bounds__(kGradWarps * 32) lowRankGradKernel(Grad p) {
   const int width = side ? p.width[1] : p.width[0];
   const long long ld = side ? p.x_ld[1] : p.x_ld[0];
   float *partial = side ? p.partial[1] : p.partial[0];
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int unit = blockIdx.y * kGradWarps + (threadIdx.x >> 5);
-  if (tile.rows <= 0 || tile.id < 0 || partial == nullptr || unit * UC >= width) {
-    return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  if (tile.rows <= 0 || tile.id < 0 || partial == nullptr || (int)blockIdx.y * kGradWarps * UC >= width) {
+    return; // all threads alike
   }
+  const int unit = blockIdx.y * kGradWarps + warp; // may lie past the width: all its columns are zeros then
   const T *x = (const T *)(side ? p.x[1] : p.x[0]) + tile.row0 * ld;
   const float *u = (side ? p.u[1] : p.u[0]) + (long long)tile.row0 * p.rank + r0;
-  const int ranks = p.rank - r0, fcol = unit * UC + NJ * g;
+  const int ranks = min(p.rank - r0, 16 * RT);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem);
+  const int chunks = (tile.rows + kGradRows - 1) / kGradRows;
+  const auto fetch = [&](int i, int stage) {
+    if (i < chunks) {
+      const uint32_t dst = ring + stage * Shape::STAGE;
+      const int row0 = i * kGradRows, rows = tile.rows - row0;
+      const int col = unit * UC + (lane & 7) * E;
+      const uint32_t mine = dst + warp * Shape::XB + (lane >> 3) * 128 + (lane & 7) * 16;
+      const T *src = x + (row0 + (lane >> 3)) * ld + col;
+#pragma unroll
+      for (int q = 0; q < kGradRows / 4; q++, src += 4 * ld) {
+        fetch16B<T, VEC>(mine + q * 512, src, col, width, q * 4 + (lane >> 3) < rows);
+      }
+      for (int e = threadIdx.x; e < kGradRows * 16 * RT; e += kGradWarps * 32) {
+        const int r = e / (16 * RT), c = e % (16 * RT);
+        const bool in = r < rows && c < ranks;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + kGradWarps * Shape::XB +
+                                                                         (r * Shape::US + c) * 4),
+                     "l"(u + (in ? (long long)(row0 + r) * p.rank + c : 0)), "r"(in ? 4 : 0)
+                     : "memory");
+      }
+    }
+    fetchCommit();
+  };
   float acc[RT][NJ][4];
 #pragma unroll
   for (int i = 0; i < RT; i++) {
@@ -547,22 +838,29 @@ __global__ void __launch_bounds__(kGradWarps * 32) lowRankGradKernel(Grad p) {
       acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
     }
   }
-#pragma unroll 4
-  for (int r = 0; r < tile.rows; r += 8) {
-    const bool in0 = r + t < tile.rows, in1 = r + t + 4 < tile.rows;
-    const uint4 none = make_uint4(0, 0, 0, 0);
-    const uint4 x0 = in0 ? load16B<T, VEC>(x + (r + t) * ld, fcol, width) : none;
-    const uint4 x1 = in1 ? load16B<T, VEC>(x + (r + t + 4) * ld, fcol, width) : none;
 #pragma unroll
-    for (int i = 0; i < RT; i++) {
-      const float *u0 = u + (long long)(r + t) * p.rank + i * 16 + g, *u1 = u0 + 4 * p.rank;
-      const bool lowr = i * 16 + g < ranks, highr = i * 16 + g + 8 < ranks;
-      uint32_t hi[4], lo[4];
-      split(in0 && lowr ? u0[0] : 0.0f, hi[0], lo[0]);
-      split(in0 && highr ? u0[8] : 0.0f, hi[1], lo[1]);
-      split(in1 && lowr ? u1[0] : 0.0f, hi[2], lo[2]);
-      split(in1 && highr ? u1[8] : 0.0f, hi[3], lo[3]);
-      mmaColumns<T, NJ>(acc[i], hi, lo, x0, x1);
+  for (int q = 0; q < S - 1; q++) {
+    fetch(q, q);
+  }
+  for (int i = 0; i < chunks; i++) {
+    fetchWait<S - 2>();
+    __syncthreads(); // chunk i is there for all, and all are done with the stage of chunk i - 1
+    fetch(i + S - 1, (i + S - 1) % S);
+    const unsigned char *src = smem + (i % S) * Shape::STAGE;
+    const float *us = reinterpret_cast<const float *>(src + kGradWarps * Shape::XB);
+#pragma unroll
+    for (int r = 0; r < kGradRows; r += 8) {
+      const uint4 x0 = shared16B(src + warp * Shape::XB + (r + t) * 128 + g * 16);
+      const uint4 x1 = shared16B(src + warp * Shape::XB + (r + t + 4) * 128 + g * 16);
+      uint32_t hi[RT][4], lo[RT][4];
+#pragma unroll
+      for (int q = 0; q < RT; q++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          split(us[(r + t + (e >> 1) * 4) * Shape::US + q * 16 + g + (e & 1) * 8], hi[q][e], lo[q][e]);
+        }
+      }
+      mmaColumns<T, false>(acc, hi, lo, x0, x1);
     }
   }
   const int col = unit * UC + 2 * NJ * t;
@@ -629,7 +927,9 @@ template <typename T, bool VEC> void launchGrad(Grad p, long long slots, cudaStr
   p.rank_passes = (p.rank + 16 * rt - 1) / (16 * rt);
   const dim3 grid((unsigned)slots, (unsigned)((widest + uc - 1) / uc), (unsigned)(2 * p.rank_passes));
   auto kernel = rt == 1 ? lowRankGradKernel<T, VEC, 1> : rt == 2 ? lowRankGradKernel<T, VEC, 2> : lowRankGradKernel<T, VEC, 4>;
-  AB200_CUDA(launchChained(kernel, grid, dim3(kGradWarps * 32), 0, st, p));
+  const int smem = rt == 1 ? GradShape<1>::BYTES : rt == 2 ? GradShape<2>::BYTES : GradShape<4>::BYTES;
+  AB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  AB200_CUDA(launchChained(kernel, grid, dim3(kGradWarps * 32), smem, st, p));
   AB200_LAUNCH_CHECK();
 }
 template <typename T>
@@ -647,7 +947,7 @@ void gradOfType(const Grad &p, const LowRankGradArgs &a, long long slots, bool v
 
 bool rowsAlign(const void *p, long long ld, int width, int type) {
   const int size = type == DT_F32 ? 4 : 2;
-  return p == nullptr || ((uintptr_t)p % 32 == 0 && ld * size % 32 == 0 && (long long)width * size % 32 == 0);
+  return p == nullptr || ((uintptr_t)p % 16 == 0 && ld * size % 16 == 0 && (long long)width * size % 16 == 0);
 }
 
 } // namespace
@@ -675,9 +975,14 @@ void lowRankApply(const LowRankArgs &a, cudaStream_t stream) {
                    rowsAlign(a.y.p, a.y.ld, a.n, a.type) && rowsAlign(a.a, a.k, a.k, a.type) &&
                    rowsAlign(a.b, a.n, a.n, a.type);
   switch (a.type) {
-  case DT_F32: dispatchApply<float>(p, a.seg, vec, stream); break;
-  case DT_F16: dispatchApply<__half>(p, a.seg, vec, stream); break;
-  default: dispatchApply<__nv_bfloat16>(p, a.seg, vec, stream);
+  case DT_F32:
+    vec ? dispatchApply<float, true>(p, a.seg, stream) : dispatchApply<float, false>(p, a.seg, stream);
+    break;
+  case DT_F16:
+    vec ? dispatchApply<__half, true>(p, a.seg, stream) : dispatchApply<__half, false>(p, a.seg, stream);
+    break;
+  default:
+    vec ? dispatchApply<__nv_bfloat16, true>(p, a.seg, stream) : dispatchApply<__nv_bfloat16, false>(p, a.seg, stream);
   }
 }
 
