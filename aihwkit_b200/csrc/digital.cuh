@@ -108,6 +108,10 @@ template <typename T, bool VEC> struct Raw8 {
     }
   }
   __device__ __forceinline__ void get(float v[8]) const { unpack8<T>(q, v); }
+  // elements whose half of the masks is zero become zero, whatever they were
+  __device__ __forceinline__ void mask(const uint32_t m[4]) {
+    q = make_uint4(q.x & m[0], q.y & m[1], q.z & m[2], q.w & m[3]);
+  }
 };
 template <bool VEC> struct Raw8<float, VEC> {
   float f[8];
@@ -163,6 +167,62 @@ __device__ __forceinline__ void storeSpan(T *row, int span, int lane, int cols, 
         row[c] = Elem<T>::put(v[i]);
       }
     }
+  }
+}
+
+// ---- rows ahead -------------------------------------------------------------------------------
+// A kernel that walks over rows fetches the next one with cp.async while it works on the present one:
+// every thread copies the elements that it will read itself into slots of its own, so no barrier and
+// no wait on other threads is needed, and the registers stay free. Two stages; a stage has a slot of 16 bytes
+// (two for fp32) per tensor, span and thread, threads side by side.
+template <typename T, int NS> struct RowRing {
+  static constexpr int PLANES = sizeof(T) == 4 ? 2 : 1;
+  const unsigned char *own; // this thread's first slot
+  int plane;                // bytes from slot to slot
+  int per_stage;            // slots
+  __device__ __forceinline__ RowRing(const void *smem, int tensors) {
+    own = (const unsigned char *)smem + threadIdx.x * 16;
+    plane = blockDim.x * 16;
+    per_stage = tensors * NS * PLANES;
+  }
+  static size_t bytes(int tensors, int threads) { return (size_t)2 * tensors * NS * PLANES * 16 * threads; }
+  __device__ __forceinline__ int slot(int stage, int tensor, int s) const {
+    return (stage * per_stage + (tensor * NS + s) * PLANES) * plane;
+  }
+  // columns past the end become zeros, without a read
+  __device__ __forceinline__ void issue(int stage, int tensor, int s, const T *row, int span, int lane, int cols) const {
+    const int c = Span<true>::col(span, lane, 0);
+    const char *src = reinterpret_cast<const char *>(row + c);
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(own + slot(stage, tensor, s));
+#pragma unroll
+    for (int h = 0; h < PLANES; h++) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + h * plane), "l"(src + 16 * h),
+                   "r"(c < cols ? 16 : 0)
+                   : "memory");
+    }
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  // all but the newest group of this thread have arrived
+  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+  __device__ __forceinline__ void get(int stage, int tensor, int s, Raw8<T, true> &r) const {
+    const unsigned char *src = own + slot(stage, tensor, s);
+    if constexpr (PLANES == 2) {
+      const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + plane);
+      r.f[0] = a.x, r.f[1] = a.y, r.f[2] = a.z, r.f[3] = a.w;
+      r.f[4] = b.x, r.f[5] = b.y, r.f[6] = b.z, r.f[7] = b.w;
+    } else {
+      r.q = *reinterpret_cast<const uint4 *>(src);
+    }
+  }
+};
+
+// pairs of 16-bit results, masked as above
+template <typename T>
+__device__ __forceinline__ void storeMasked(T *row, int span, int lane, int cols, const float v[8], const uint32_t m[4]) {
+  const int c = Span<true>::col(span, lane, 0);
+  if (c < cols) {
+    *reinterpret_cast<uint4 *>(row + c) = make_uint4(pack2<T>(v[0], v[1]) & m[0], pack2<T>(v[2], v[3]) & m[1],
+                                                     pack2<T>(v[4], v[5]) & m[2], pack2<T>(v[6], v[7]) & m[3]);
   }
 }
 
@@ -279,6 +339,13 @@ __device__ __forceinline__ Kept keepOfSpan(const DropKey &k, long long row, int 
     }
   }
   return mine;
+}
+// masks of the pairs of 16-bit elements: a quarter of the masks of eight floats
+__device__ __forceinline__ void pairMasks(const Kept &kept, uint32_t m[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    m[i] = signMask(kept.w[i], 0xbb99);
+  }
 }
 // v = kept ? v * scale : 0, whatever v is
 __device__ __forceinline__ void dropSpan(const DropKey &k, const Kept &kept, float v[8]) {

@@ -61,16 +61,13 @@ __global__ void __launch_bounds__(256)
       const Kept kept = keepOfSpan<VEC>(key, row[q], span[q], lane, cols);
       raw[q].get(v);
       if constexpr (VEC && !RES && sizeof(T) == 2) {
-        // pairs of results are masked as they are stored, a quarter of the masks
-        const int c = Span<true>::col(span[q], lane, 0);
-        if (c < cols) {
-          uint32_t o[4];
+        uint32_t m[4];
+        pairMasks(kept, m);
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            o[i] = pack2<T>(v[2 * i] * key.scale, v[2 * i + 1] * key.scale) & signMask(kept.w[i], 0xbb99);
-          }
-          *reinterpret_cast<uint4 *>(y + row[q] * y_ld + c) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int i = 0; i < 8; i++) {
+          v[i] *= key.scale;
         }
+        storeMasked(y + row[q] * y_ld, span[q], lane, cols, v, m);
       } else {
         dropSpan(key, kept, v);
         if (RES) {
