@@ -16,7 +16,8 @@
 // through distributed shared memory in rank order, and each block takes a share of the columns.
 // Products: bf16 x bf16 and fp16 x fp16 are exact in the fp32 sum; fp32 factors (v, and x, a, b of
 // fp32 calls) are split into two TF32 parts, hi + lo, and multiplied as hi hi + lo hi + hi lo, which leaves
-// 2^-22 of a product out.
+// 2^-22 of a product out. Where v (or u of the gradients) meets bf16, its two parts are bf16: 16 bits of it, 2^-17 off
+// against the 2^-9 of the rounding of the result, for half the products. fp16 has not the range for that.
 //
 // lowRankGradKernel. grad[id] = sum over the rows of id of u^T x: a warp holds rank x 128 bytes of columns
 // in fragments and walks a chunk of rows of one request, fetched the same way; chunks' partial sums go
@@ -175,6 +176,14 @@ __device__ __forceinline__ void split(float v, uint32_t &hi, uint32_t &lo) {
   lo = __float_as_uint(v - __uint_as_float(hi));
 }
 
+// a and b as the halves of a word, in bf16, and what is left of them in another
+__device__ __forceinline__ void splitPair(float a, float b, uint32_t &hi, uint32_t &lo) {
+  hi = pack2<__nv_bfloat16>(a, b);
+  const float2 f = unpack2<__nv_bfloat16>(hi);
+  lo = pack2<__nv_bfloat16>(a - f.x, b - f.y);
+}
+template <typename T> constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
+
 // 16 bytes of a row: eight 16-bit or four fp32 neighbours; elements past the end read as zero
 template <typename T, bool VEC>
 __device__ __forceinline__ uint4 load16B(const T *p, int col, int cols) {
@@ -289,25 +298,77 @@ __device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], const uint32
   }
 }
 
+// The same for bf16 and sixteen rows of the factor: rows t and t + 4 (b[0], b[1]) go as a pair, and rows t + 8 and
+// t + 12 (b[2], b[3]); hi and lo hold their factors in the same pairs
+template <bool FIRST, int MT, int NJ>
+__device__ __forceinline__ void mmaPairs(float (&acc)[MT][NJ][4], const uint32_t (&hi)[MT][4], const uint32_t (&lo)[MT][4],
+                                         const uint4 (&b)[4]) {
+  uint32_t p[NJ][2];
+#pragma unroll
+  for (int j = 0; j < NJ; j++) {
+    const int w = j >> 1;
+    const uint32_t pick = (j & 1) ? 0x7632 : 0x5410; // high or low halves of two words
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint4 &x = b[2 * h], &y = b[2 * h + 1];
+      p[j][h] = __byte_perm(w == 0 ? x.x : w == 1 ? x.y : w == 2 ? x.z : x.w, w == 0 ? y.x : w == 1 ? y.y : w == 2 ? y.z : y.w, pick);
+    }
+  }
+#pragma unroll
+  for (int term = 0; term < 2; term++) {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        if (FIRST && term == 0) {
+          acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
+        }
+        mma16<__nv_bfloat16>(acc[i][j], term == 0 ? lo[i] : hi[i], p[j][0], p[j][1]);
+      }
+    }
+  }
+}
+
 // ---- rings of cp.async ------------------------------------------------------------------------
 // 16 bytes of a row to shared memory, from `src`, the place of column `col`; columns past the end, and all
-// of them where `in` is false, become zeros without a read (nor a branch). Rows that 16-byte
-// accesses do not fit go by elements: fp32 still asynchronously, 16-bit ones through registers.
+// of them where `in` is false, become zeros without a read (nor a branch). fp32 rows that 16-byte
+// accesses do not fit go by elements, 16-bit ones through registers (fetchRows).
 template <typename T, bool VEC>
 __device__ __forceinline__ void fetch16B(uint32_t dst, const T *src, int col, int cols, bool in) {
   if (VEC) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in && col < cols ? 16 : 0)
                  : "memory");
-  } else if constexpr (sizeof(T) == 4) {
+  } else {
+    static_assert(VEC || sizeof(T) == 4, "16-bit elements are below what cp.async copies");
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * i), "l"(src + i),
                    "r"(in && col + i < cols ? 4 : 0)
                    : "memory");
     }
+  }
+}
+// N such pieces, of rows `step` elements apart and STRIDE bytes apart in shared memory, of which the first
+// `rows` are there in steps of EVERY from row `first`; what goes through registers is read before any of it is stored
+template <typename T, bool VEC, int N, int STRIDE, int EVERY>
+__device__ __forceinline__ void fetchRows(uint32_t dst, const T *src, long long step, int col, int cols, int first, int rows) {
+  if constexpr (VEC || sizeof(T) == 4) {
+#pragma unroll
+    for (int q = 0; q < N; q++, src += step) {
+      fetch16B<T, VEC>(dst + q * STRIDE, src, col, cols, q * EVERY + first < rows);
+    }
   } else {
-    const uint4 q = load16B<T, false>(src - col, col, in ? cols : 0);
-    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+    uint4 piece[N];
+#pragma unroll
+    for (int q = 0; q < N; q++, src += step) {
+      piece[q] = load16B<T, false>(src - col, col, q * EVERY + first < rows ? cols : 0);
+    }
+#pragma unroll
+    for (int q = 0; q < N; q++) {
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + q * STRIDE), "r"(piece[q].x), "r"(piece[q].y),
+                   "r"(piece[q].z), "r"(piece[q].w)
+                   : "memory");
+    }
   }
 }
 __device__ __forceinline__ void fetchCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -437,7 +498,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   const int r_pad = (p.rank + 7) & ~7, vs = r_pad + 4;
   const unsigned char *held = smem + warp * S * Shape::STAGE; // this warp's ring, as it is read
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(held);
-  // v of the tile as the second product's operands: [fragment][8 ranks][hi, lo][lane][4]
+  // v of the tile as the second product's operands: [fragment][8 ranks (bf16: 16)][hi, lo][lane][4]
   float *v = reinterpret_cast<float *>(smem + Shape::RING);
   float *mine = v + TM * r_pad * 2; // [TM][vs]: this block's share of v
   float *shares = mine + TM * vs;   // [W][TM][RC + 4], of tiles of 16 rows
@@ -469,17 +530,10 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
       const uint32_t dst = ring + f_stage * Shape::STAGE + own;
       const bool last = f_rank + RC >= p.rank;
       if (p.base != nullptr && last) {
-        const T *src = base_at + c0;
-#pragma unroll
-        for (int q = 0; q < 2 * MT; q++, src += base_8) {
-          fetch16B<T, VEC>(dst + q * 512, src, col, p.n, q * 8 + g < rows_in);
-        }
+        fetchRows<T, VEC, 2 * MT, 512, 8>(dst, base_at + c0, base_8, col, p.n, g, rows_in);
       }
-      const T *src = fb + (long long)(f_rank + g) * p.n + col;
-#pragma unroll
-      for (int j = 0; j < NT; j++, src += 8 * p.n) {
-        fetch16B<T, VEC>(dst + Shape::XB + j * 512, src, col, p.n, f_rank + j * 8 + g < p.rank);
-      }
+      fetchRows<T, VEC, NT, 512, 8>(dst + Shape::XB, fb + (long long)(f_rank + g) * p.n + col, 8LL * p.n, col, p.n, f_rank + g,
+                                    p.rank);
       f_rank = last ? 0 : f_rank + RC;
       f_unit += last ? W : 0;
     }
@@ -499,16 +553,8 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
       if (s < s_end) {
         const int c0 = s * KS, k0 = c0 + t * E;
         const uint32_t dst = ring + stage * Shape::STAGE + own_x;
-        const T *src = x_at + c0;
-#pragma unroll
-        for (int q = 0; q < 2 * MT; q++, src += x_8) {
-          fetch16B<T, VEC>(dst + q * 512, src, k0, p.k, q * 8 + g < rows_in);
-        }
-        const T *f = fa + (long long)(r0 + g) * p.k + k0;
-#pragma unroll
-        for (int j = 0; j < NT; j++, f += 8 * p.k) {
-          fetch16B<T, VEC>(dst + Shape::XB + j * 512, f, k0, p.k, r0 + j * 8 + g < p.rank);
-        }
+        fetchRows<T, VEC, 2 * MT, 512, 8>(dst, x_at + c0, x_8, k0, p.k, g, rows_in);
+        fetchRows<T, VEC, NT, 512, 8>(dst + Shape::XB, fa + (long long)(r0 + g) * p.k + k0, 8LL * p.k, k0, p.k, r0 + g, p.rank);
       }
       fetchCommit();
     };
@@ -599,10 +645,12 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   if (p.cluster > 1) {
     cluster.sync();
   }
+  const int c_end = kPairs<T> ? (p.rank + 15) & ~15 : r_pad; // pairs come in sixteens of ranks
   for (int r = threadIdx.x / 8; r < TM; r += W * 4) {
-    for (int c = threadIdx.x % 8; c < r_pad; c += 8) {
+    for (int c = threadIdx.x % 8; c < c_end; c += 8) {
       float sum = 0.0f;
-      if (p.cluster > 1) {
+      if (c >= r_pad) {
+      } else if (p.cluster > 1) {
         float share[8]; // all on their way before the first is added
 #pragma unroll
         for (int q = 0; q < 8; q++) {
@@ -616,11 +664,20 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
         sum = mine[r * vs + c];
       }
       sum *= scale;
-      uint32_t hi, lo;
-      split(sum, hi, lo);
-      float *d = v + ((r / 16 * (r_pad / 8) + c / 8) * 64 + r % 8 * 4 + c % 4) * 4 + (r % 16) / 8 + (c % 8) / 4 * 2;
-      d[0] = __uint_as_float(hi);
-      d[128] = __uint_as_float(lo);
+      if constexpr (kPairs<T>) {
+        const __nv_bfloat16 hi = __float2bfloat16_rn(sum);
+        __nv_bfloat16 *d = reinterpret_cast<__nv_bfloat16 *>(v) +
+                           (((r / 16 * (c_end / 16) + c / 16) * 64 + r % 8 * 4 + c % 4) * 4 + (r % 16) / 8 + (c % 16) / 8 * 2) * 2 +
+                           (c % 8) / 4;
+        d[0] = hi;
+        d[256] = __float2bfloat16_rn(sum - __bfloat162float(hi));
+      } else {
+        uint32_t hi, lo;
+        split(sum, hi, lo);
+        float *d = v + ((r / 16 * (r_pad / 8) + c / 8) * 64 + r % 8 * 4 + c % 4) * 4 + (r % 16) / 8 + (c % 8) / 4 * 2;
+        d[0] = __uint_as_float(hi);
+        d[128] = __uint_as_float(lo);
+      }
       if (p.v != nullptr && part == 0 && r < tile.rows && c < p.rank) {
         const long long row = MT == 1 ? tile_rows[warp][r] : tile.row0 + r;
         p.v[row * p.rank + c] = sum;
@@ -651,28 +708,36 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
     __syncwarp(); // b is read by other lanes than fetched it
     const unsigned char *src = held + stage * Shape::STAGE;
     stage = stage + 1 == S ? 0 : stage + 1;
-    const auto ranks8 = [&](int r, auto first) {
-      const uint4 b0 = shared8B(src + Shape::XB + (r + t) * 64 + g * 8);
-      const uint4 b1 = shared8B(src + Shape::XB + (r + t + 4) * 64 + g * 8);
+    constexpr int RS = kPairs<T> ? 16 : 8; // ranks to a product
+    const auto ranks = [&](int r, auto first) {
       uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
       for (int m = 0; m < MT; m++) {
-        const uint4 *q = operands + (m * (r_pad / 8) + (r0 + r) / 8) * 64;
+        const uint4 *q = operands + (m * (c_end / RS) + (r0 + r) / RS) * 64;
         const uint4 qh = q[0], ql = q[32];
         hi[m][0] = qh.x, hi[m][1] = qh.y, hi[m][2] = qh.z, hi[m][3] = qh.w;
         lo[m][0] = ql.x, lo[m][1] = ql.y, lo[m][2] = ql.z, lo[m][3] = ql.w;
       }
-      mmaColumns<T, decltype(first)::value>(acc, hi, lo, b0, b1);
+      uint4 b[RS / 4];
+#pragma unroll
+      for (int q = 0; q < RS / 4; q++) {
+        b[q] = r + q * 4 < RC ? shared8B(src + Shape::XB + (r + q * 4 + t) * 64 + g * 8) : make_uint4(0, 0, 0, 0);
+      }
+      if constexpr (kPairs<T>) {
+        mmaPairs<decltype(first)::value>(acc, hi, lo, b);
+      } else {
+        mmaColumns<T, decltype(first)::value>(acc, hi, lo, b[0], b[1]);
+      }
     };
     if (r0 == 0) {
-      ranks8(0, std::true_type());
+      ranks(0, std::true_type());
     } else {
-      ranks8(0, std::false_type());
+      ranks(0, std::false_type());
     }
 #pragma unroll
-    for (int r = 8; r < RC; r += 8) {
-      if (r0 + r < r_pad) {
-        ranks8(r, std::false_type());
+    for (int r = RS; r < RC; r += RS) {
+      if (r0 + r < p.rank) {
+        ranks(r, std::false_type());
       }
     }
     if (r0 + RC < p.rank) {
@@ -806,6 +871,7 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
   const T *x = (const T *)(side ? p.x[1] : p.x[0]) + tile.row0 * ld;
   const float *u = (side ? p.u[1] : p.u[0]) + (long long)tile.row0 * p.rank + r0;
   const int ranks = min(p.rank - r0, 16 * RT);
+  const bool u_wide = p.rank % 4 == 0 && (uintptr_t)u % 16 == 0;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem);
   const int chunks = (tile.rows + kGradRows - 1) / kGradRows;
   const auto fetch = [&](int i, int stage) {
@@ -814,18 +880,21 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
       const int row0 = i * kGradRows, rows = tile.rows - row0;
       const int col = unit * UC + (lane & 7) * E;
       const uint32_t mine = dst + warp * Shape::XB + (lane >> 3) * 128 + (lane & 7) * 16;
-      const T *src = x + (row0 + (lane >> 3)) * ld + col;
-#pragma unroll
-      for (int q = 0; q < kGradRows / 4; q++, src += 4 * ld) {
-        fetch16B<T, VEC>(mine + q * 512, src, col, width, q * 4 + (lane >> 3) < rows);
-      }
-      for (int e = threadIdx.x; e < kGradRows * 16 * RT; e += kGradWarps * 32) {
-        const int r = e / (16 * RT), c = e % (16 * RT);
-        const bool in = r < rows && c < ranks;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + kGradWarps * Shape::XB +
-                                                                         (r * Shape::US + c) * 4),
-                     "l"(u + (in ? (long long)(row0 + r) * p.rank + c : 0)), "r"(in ? 4 : 0)
-                     : "memory");
+      fetchRows<T, VEC, kGradRows / 4, 512, 4>(mine, x + (row0 + (lane >> 3)) * ld + col, 4 * ld, col, width, lane >> 3, rows);
+      if (u_wide) {
+        for (int e = threadIdx.x; e < kGradRows * 4 * RT; e += kGradWarps * 32) {
+          const int r = e / (4 * RT), c = e % (4 * RT) * 4;
+          fetch16B<float, true>(dst + kGradWarps * Shape::XB + (r * Shape::US + c) * 4, u + (long long)(row0 + r) * p.rank + c,
+                                c, ranks, r < rows);
+        }
+      } else {
+        for (int e = threadIdx.x; e < kGradRows * 16 * RT; e += kGradWarps * 32) {
+          const int r = e / (16 * RT), c = e % (16 * RT);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + kGradWarps * Shape::XB +
+                                                                           (r * Shape::US + c) * 4),
+                       "l"(u + (long long)(row0 + r) * p.rank + c), "r"(r < rows && c < ranks ? 4 : 0)
+                       : "memory");
+        }
       }
     }
     fetchCommit();
@@ -848,19 +917,41 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
     fetch(i + S - 1, (i + S - 1) % S);
     const unsigned char *src = smem + (i % S) * Shape::STAGE;
     const float *us = reinterpret_cast<const float *>(src + kGradWarps * Shape::XB);
+    const unsigned char *xs = src + warp * Shape::XB + t * 128 + g * 16;
+    const float *uf = us + t * Shape::US + g;
+    if constexpr (kPairs<T>) {
 #pragma unroll
-    for (int r = 0; r < kGradRows; r += 8) {
-      const uint4 x0 = shared16B(src + warp * Shape::XB + (r + t) * 128 + g * 16);
-      const uint4 x1 = shared16B(src + warp * Shape::XB + (r + t + 4) * 128 + g * 16);
-      uint32_t hi[RT][4], lo[RT][4];
+      for (int r = 0; r < kGradRows; r += 16) {
+        uint4 b[4];
 #pragma unroll
-      for (int q = 0; q < RT; q++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          split(us[(r + t + (e >> 1) * 4) * Shape::US + q * 16 + g + (e & 1) * 8], hi[q][e], lo[q][e]);
+        for (int q = 0; q < 4; q++) {
+          b[q] = shared16B(xs + (r + 4 * q) * 128);
         }
+        uint32_t hi[RT][4], lo[RT][4];
+#pragma unroll
+        for (int q = 0; q < RT; q++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float *f = uf + (r + (e >> 1) * 8) * Shape::US + q * 16 + (e & 1) * 8;
+            splitPair(f[0], f[4 * Shape::US], hi[q][e], lo[q][e]);
+          }
+        }
+        mmaPairs<false>(acc, hi, lo, b);
       }
-      mmaColumns<T, false>(acc, hi, lo, x0, x1);
+    } else {
+#pragma unroll
+      for (int r = 0; r < kGradRows; r += 8) {
+        const uint4 x0 = shared16B(xs + r * 128), x1 = shared16B(xs + (r + 4) * 128);
+        uint32_t hi[RT][4], lo[RT][4];
+#pragma unroll
+        for (int q = 0; q < RT; q++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            split(uf[(r + (e >> 1) * 4) * Shape::US + q * 16 + (e & 1) * 8], hi[q][e], lo[q][e]);
+          }
+        }
+        mmaColumns<T, false>(acc, hi, lo, x0, x1);
+      }
     }
   }
   const int col = unit * UC + 2 * NJ * t;
@@ -882,34 +973,65 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
   }
 }
 
-// grad[i] = sum of the partial sums of adapter i's chunks, in the order of the rows; zero without any
-template <typename T>
-__global__ void __launch_bounds__(256)
+// grad[i] = sum of the partial sums of adapter i's chunks; zero without any. A warp has 32 elements; where
+// elements are few, the warps of a block share them (SHARED), warp w taking the adapter's chunks w, w + 8, ... The
+// chunks go in the order of the rows, so the order of the sum is fixed.
+constexpr int kJoinWarps = 8;
+template <typename T, bool SHARED>
+__global__ void __launch_bounds__(kJoinWarps * 32)
     lowRankJoinKernel(const int *__restrict__ slot_id, int slots, const float *__restrict__ p0,
                       const float *__restrict__ p1, T *g0, T *g1, long long elems0, long long elems1) {
   pdlEnter();
-  const int side = blockIdx.z, i = blockIdx.y;
+  __shared__ float part[kJoinWarps][32];
+  const int side = blockIdx.z, i = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long elems = side ? elems1 : elems0;
   const float *partial = side ? p1 : p0;
   T *grad = side ? g1 : g0;
-  const long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (grad == nullptr || e >= elems) {
+  const long long e = ((long long)blockIdx.x * (SHARED ? 1 : kJoinWarps) + (SHARED ? 0 : warp)) * 32 + lane;
+  if (grad == nullptr) {
     return;
   }
+  const float *mine = partial + (e < elems ? e : 0);
   float sum = 0.0f;
-  for (int s = 0; s < slots; s++) {
-    if (slot_id[s] == i) {
-      sum += partial[s * elems + e];
+  int seen = 0; // chunks of the adapter before these 32
+  for (int s0 = 0; s0 < slots; s0 += 32) {
+    unsigned left = __ballot_sync(0xffffffffu, s0 + lane < slots && slot_id[s0 + lane] == i);
+    while (left != 0) {
+      float v[4]; // four chunks on their way before the first is added
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const bool take = left != 0 && (!SHARED || seen % kJoinWarps == warp);
+        v[q] = take ? mine[(long long)(s0 + __ffs(left) - 1) * elems] : 0.0f;
+        seen += left != 0 ? 1 : 0;
+        left &= left - 1;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        sum += v[q];
+      }
     }
   }
-  grad[i * elems + e] = Elem<T>::put(sum);
+  if (SHARED) {
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp != 0) {
+      return;
+    }
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; w++) {
+      sum += part[w][lane];
+    }
+  }
+  if (e < elems) {
+    grad[i * elems + e] = Elem<T>::put(sum);
+  }
 }
 
-// rows per chunk: enough blocks for three per multiprocessor, between 32 and 2048 rows
+// rows per chunk: enough blocks for two per multiprocessor, between 128 and 2048 rows
 int gradShift(const LowRankRows &s, int width0, int width1) {
   int shift = 11;
   const long long units = (width0 + width1 + 255) / 256;
-  while (shift > 5 && units * (s.rows >> shift) < 3LL * digitalSmCount()) {
+  while (shift > 7 && units * (s.rows >> shift) < 2LL * digitalSmCount()) {
     shift--;
   }
   return shift;
@@ -939,8 +1061,11 @@ void gradOfType(const Grad &p, const LowRankGradArgs &a, long long slots, bool v
   }
   const long long e0 = (long long)a.rank * a.width[0], e1 = (long long)a.rank * a.width[1];
   const long long most = std::max(a.grad[0] ? e0 : 0, a.grad[1] ? e1 : 0);
-  AB200_CUDA(launchChained(lowRankJoinKernel<T>, dim3((unsigned)((most + 255) / 256), (unsigned)a.adapters, 2), dim3(256),
-                           0, st, (const int *)p.slot_id, (int)slots, (const float *)p.partial[0],
+  const long long warps = (most + 31) / 32;
+  const bool shared = warps * a.adapters < 4LL * digitalSmCount();
+  auto join = shared ? lowRankJoinKernel<T, true> : lowRankJoinKernel<T, false>;
+  AB200_CUDA(launchChained(join, dim3((unsigned)(shared ? warps : (warps + kJoinWarps - 1) / kJoinWarps), (unsigned)a.adapters, 2),
+                           dim3(kJoinWarps * 32), 0, st, (const int *)p.slot_id, (int)slots, (const float *)p.partial[0],
                            (const float *)p.partial[1], (T *)a.grad[0], (T *)a.grad[1], e0, e1));
   AB200_LAUNCH_CHECK();
 }
