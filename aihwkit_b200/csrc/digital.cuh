@@ -171,48 +171,35 @@ __device__ __forceinline__ void storeSpan(T *row, int span, int lane, int cols, 
 }
 
 // ---- rows ahead -------------------------------------------------------------------------------
-// A kernel that walks over rows fetches the next one with cp.async while it works on the present one:
+// A kernel that walks over 16-bit rows fetches the next one with cp.async while it works on the present one:
 // every thread copies the elements that it will read itself into slots of its own, so no barrier and
 // no wait on other threads is needed, and the registers stay free. Two stages; a stage has a slot of 16 bytes
-// (two for fp32) per tensor, span and thread, threads side by side.
+// per tensor, span and thread, threads side by side.
 template <typename T, int NS> struct RowRing {
-  static constexpr int PLANES = sizeof(T) == 4 ? 2 : 1;
   const unsigned char *own; // this thread's first slot
   int plane;                // bytes from slot to slot
   int per_stage;            // slots
   __device__ __forceinline__ RowRing(const void *smem, int tensors) {
     own = (const unsigned char *)smem + threadIdx.x * 16;
     plane = blockDim.x * 16;
-    per_stage = tensors * NS * PLANES;
+    per_stage = tensors * NS;
   }
-  static size_t bytes(int tensors, int threads) { return (size_t)2 * tensors * NS * PLANES * 16 * threads; }
+  static size_t bytes(int tensors, int threads) { return (size_t)2 * tensors * NS * 16 * threads; }
   __device__ __forceinline__ int slot(int stage, int tensor, int s) const {
-    return (stage * per_stage + (tensor * NS + s) * PLANES) * plane;
+    return (stage * per_stage + tensor * NS + s) * plane;
   }
   // columns past the end become zeros, without a read
   __device__ __forceinline__ void issue(int stage, int tensor, int s, const T *row, int span, int lane, int cols) const {
     const int c = Span<true>::col(span, lane, 0);
-    const char *src = reinterpret_cast<const char *>(row + c);
     const uint32_t dst = (uint32_t)__cvta_generic_to_shared(own + slot(stage, tensor, s));
-#pragma unroll
-    for (int h = 0; h < PLANES; h++) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + h * plane), "l"(src + 16 * h),
-                   "r"(c < cols ? 16 : 0)
-                   : "memory");
-    }
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(row + c), "r"(c < cols ? 16 : 0)
+                 : "memory");
   }
   static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
   // all but the newest group of this thread have arrived
   static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
   __device__ __forceinline__ void get(int stage, int tensor, int s, Raw8<T, true> &r) const {
-    const unsigned char *src = own + slot(stage, tensor, s);
-    if constexpr (PLANES == 2) {
-      const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + plane);
-      r.f[0] = a.x, r.f[1] = a.y, r.f[2] = a.z, r.f[3] = a.w;
-      r.f[4] = b.x, r.f[5] = b.y, r.f[6] = b.z, r.f[7] = b.w;
-    } else {
-      r.q = *reinterpret_cast<const uint4 *>(src);
-    }
+    r.q = *reinterpret_cast<const uint4 *>(own + slot(stage, tensor, s));
   }
 };
 

@@ -7,6 +7,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <sstream>
 #include <stdexcept>
@@ -145,30 +146,24 @@ struct Wanted {
   size_t next;
   bool operator()(const Tensor &input) { return input.defined() && ctx->needs_input_grad(next++); }
 };
-// gradients of a backward pass that is itself recorded: using them raises, as they are not
-// differentiable again
-variable_list once(variable_list grads) {
+// Gradients of a backward pass that is itself recorded: differentiating them by anything that they were made
+// from raises.
+variable_list once(variable_list grads, const variable_list &made_from) {
   if (!at::GradMode::is_enabled()) {
     return grads;
   }
-  variable_list given;
-  std::vector<size_t> where;
-  for (size_t i = 0; i < grads.size(); i++) {
-    if (grads[i].defined()) {
-      given.push_back(grads[i].detach().requires_grad_(true));
-      where.push_back(i);
+  auto node = std::make_shared<torch::autograd::Error>("the digital operators' gradients are not differentiable again",
+                                                       torch::autograd::collect_next_edges(made_from));
+  for (Tensor &g : grads) {
+    if (g.defined() && !g.requires_grad()) { // one that is passed on has its own history, one that appears twice has it by now
+      torch::autograd::set_history(g, node);
     }
   }
-  if (given.empty()) {
-    return grads;
-  }
-  auto node = std::make_shared<torch::autograd::DelayedError>(
-      "the digital operators' gradients are not differentiable again", (int64_t)given.size());
-  given = (*node)(std::move(given));
-  for (size_t i = 0; i < where.size(); i++) {
-    grads[where[i]] = given[i];
-  }
   return grads;
+}
+variable_list joined(variable_list a, const variable_list &b) {
+  a.insert(a.end(), b.begin(), b.end());
+  return a;
 }
 
 // ---- dropout ----------------------------------------------------------------------------------
@@ -197,7 +192,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
                       (uint32_t)ctx->saved_data["call"].toInt()};
     Tensor dx;
     if (ctx->needs_input_grad(0)) {
-      dx = once({dropoutCompute(gs[0], r, Tensor())})[0];
+      dx = once({dropoutCompute(gs[0], r, Tensor())}, gs)[0];
     }
     const bool need_res = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1);
     return {dx, need_res ? gs[0] : Tensor(), Tensor(), Tensor(), Tensor()};
@@ -314,7 +309,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const bool need_w = wanted(s[1]), need_b = wanted(s[2]);
     const NormGrads g = normGradCompute(gs[0], Tensor(), s[0], Tensor(), s[1], s[2], s[3], {0.0, 0, 0},
                                         ctx->needs_input_grad(0), false, need_w, need_b);
-    return once({g.dh, g.dw, g.db, Tensor()});
+    return once({g.dh, g.dw, g.db, Tensor()}, joined(gs, {s[0], s[1]}));
   }
 };
 // h = residual + dropout(x), y = norm(h). The backward pass needs h as it went into the norm: an fp32 h is
@@ -351,7 +346,8 @@ struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
         g.dx = dropoutCompute(gs[1], r, Tensor());
       }
     }
-    variable_list out = once({need_x ? (dropped ? g.dx : g.dh) : Tensor(), need_res ? g.dh : Tensor(), g.dw, g.db});
+    variable_list out = once({need_x ? (dropped ? g.dx : g.dh) : Tensor(), need_res ? g.dh : Tensor(), g.dw, g.db},
+                             joined(gs, {s[0], s[1], s[2]}));
     out.resize(8);
     return out;
   }
@@ -434,7 +430,7 @@ struct LowRankAdd : torch::autograd::Function<LowRankAdd> {
                                 (int)n, ids.data_ptr<int>(), (const int32_t *)ptr(starts), (int)ids.numel(), rows,
                                 (int)rank, (int)a.size(0), typeCode(gy, "gy"), ptr(work), stream()));
     }
-    const variable_list g = once({dx, da, db});
+    const variable_list g = once({dx, da, db}, joined(gs, {x, a, b}));
     return {ctx->needs_input_grad(0) ? gy : Tensor(), g[0], g[1], g[2], Tensor(), Tensor(), Tensor()};
   }
 };

@@ -225,8 +225,11 @@ struct NormBwd {
   int drop; // x is dropped before the sum
 };
 
-// rows are fetched ahead by blocks of few warps on long rows, where the registers leave room for no third block
-constexpr bool normAhead(bool vec, bool wide, int ns) { return vec && wide && ns == 2; }
+// 16-bit rows are fetched ahead by blocks of few warps on long rows, where the registers leave room for no third
+// block; fp32 ones of four tensors would not fit shared memory at 8192 columns
+template <typename T> constexpr bool normAhead(bool vec, bool wide, int ns) {
+  return vec && wide && ns == 2 && sizeof(T) == 2;
+}
 __host__ __device__ inline int normTensors(const NormBwd &a) { return 2 + (a.res ? 1 : 0) + (a.gh ? 1 : 0); }
 
 // Blocks walk over the rows with a fixed stride and keep the sums of the parameters' gradients of
@@ -235,7 +238,7 @@ __host__ __device__ inline int normTensors(const NormBwd &a) { return 2 + (a.res
 template <typename T, bool VEC, bool WIDE, int NS>
 __global__ void __launch_bounds__(WIDE ? 512 : kRowThreads, WIDE && NS == 1 ? 2 : 1)
     normBackwardKernel(NormBwd a, NormShape sh, DropKey key) {
-  constexpr bool AHEAD = normAhead(VEC, WIDE, NS);
+  constexpr bool AHEAD = normAhead<T>(VEC, WIDE, NS);
   pdlEnter();
   __shared__ float2 red[2][32];
   // the rows ahead; where a block has several rows, [2][cols] for its sums at the end
@@ -499,7 +502,7 @@ void launchForward(const NormShape &sh, const NormFwd &a, const DropKey &key, cu
 }
 template <typename T, bool VEC, bool WIDE, int NS>
 void launchBackward(const NormShape &sh, const NormBwd &a, const DropKey &key, int blocks, cudaStream_t stream) {
-  const size_t smem = normAhead(VEC, WIDE, NS)  ? RowRing<T, NS>::bytes(normTensors(a), normThreads(sh))
+  const size_t smem = normAhead<T>(VEC, WIDE, NS)  ? RowRing<T, NS>::bytes(normTensors(a), normThreads(sh))
                       : a.partial && !WIDE ? (size_t)sh.cols * 2 * sizeof(float)
                                            : 0;
   if (smem > 48 * 1024) {

@@ -35,6 +35,10 @@ namespace ab200 {
 
 namespace {
 
+// These kernels wait for the launch in front of them as the others do, but let the next one start only as they end: blocks
+// of a next launch that come early take the places that are free, on few multiprocessors, and stay there.
+__device__ __forceinline__ void waitForLaunchBefore() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- segments ---------------------------------------------------------------------------------
 // Rows are cut at the borders of the requests and then into tiles of 2^shift rows. With the
 // borders c(0) = 0, c(1..n+1) = starts, c(n+2) = rows, segment j owns the tile slots from
@@ -423,7 +427,7 @@ struct Apply {
 template <int MT, int NT> struct ApplyShape {
   static constexpr int TM = 16 * MT, RC = 8 * NT, W = MT == 1 ? 8 : 4;
   static constexpr int XB = TM * 64, STAGE = XB + RC * 64;
-  static constexpr int STAGES = MT == 4 || NT == 8 ? 2 : MT == 2 || NT == 4 ? 3 : 4;
+  static constexpr int STAGES = MT > 1 ? 2 : NT == 4 || NT == 8 ? 3 : 4;
   static constexpr int RING = W * STAGES * STAGE;
   // shares of the warps of a tile of 16 rows, added after one barrier; larger tiles add them in turn
   static constexpr int SHARES = MT == 1 ? W * TM * (RC + 4) * 4 : 0;
@@ -442,7 +446,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   constexpr int E = 16 / sizeof(T), KS = 4 * E; // elements in 16 bytes, of k in a step, of columns in a unit
   constexpr int NJ = E / 2;                     // fragments beside each other in a unit
   extern __shared__ __align__(16) unsigned char smem[];
-  pdlEnter();
+  waitForLaunchBefore();
   const int part = p.cluster > 1 ? blockIdx.x % p.cluster : 0;
   RowTile tile = findTile(p.seg, blockIdx.x / p.cluster);
   if (tile.rows <= 0) {
@@ -770,6 +774,8 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   }
 }
 
+constexpr long long kSharedPerSm = 228 * 1024; // of which each block takes 1 KB besides its own
+
 template <typename T, bool VEC, int MT, int NT>
 void launchApply(Apply p, const LowRankRows &seg, int shift, cudaStream_t stream) {
   p.seg.shift = shift;
@@ -777,11 +783,12 @@ void launchApply(Apply p, const LowRankRows &seg, int shift, cudaStream_t stream
   // Blocks that share a tile: as many as fit the GPU at once, eight at most. Of tiles of one row, those
   // that find others of their adapter make one; of 256 rows with 64 adapters about 80 stay.
   const long long active = MT == 1 ? std::min(slots, p.seg.adapters + slots / 16) : slots;
+  const size_t smem = ApplyShape<MT, NT>::bytes(p.rank);
+  const long long fit = std::min<long long>(ApplyShape<MT, NT>::BLOCKS, kSharedPerSm / (smem + 1024));
   p.cluster = 1;
-  while (p.cluster < 8 && active * p.cluster * 2 <= (long long)ApplyShape<MT, NT>::BLOCKS * digitalSmCount()) {
+  while (p.cluster < 8 && active * p.cluster * 2 <= fit * digitalSmCount()) {
     p.cluster *= 2;
   }
-  const size_t smem = ApplyShape<MT, NT>::bytes(p.rank);
   auto kernel = lowRankApplyKernel<T, VEC, MT, NT>;
   if (smem > 48 * 1024) {
     AB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -805,7 +812,7 @@ void launchApply(Apply p, const LowRankRows &seg, int shift, cudaStream_t stream
 template <typename T, bool VEC> void dispatchApply(const Apply &p, const LowRankRows &seg, cudaStream_t st) {
   // Requests of 16 rows and fewer on average (decoding) take tiles of 16 rows, longer ones of 64, or 32 with
   // more than 16 ranks: with the fragments of 64 rows only three blocks fitted a multiprocessor (8192 rows,
-  // 4096 -> 4096, rank 32, bf16: 78 us, 65 with 32 rows and one stage more)
+  // 4096 -> 4096, rank 32, bf16: 78 us, 51 with 32 rows)
   if (seg.starts == nullptr || seg.rows <= 16LL * seg.segments) {
     if (p.rank <= 8) {
       launchApply<T, VEC, 1, 1>(p, seg, 4, st);
@@ -854,7 +861,7 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
   using Shape = GradShape<RT>;
   constexpr int E = 16 / sizeof(T), NJ = E, UC = 8 * NJ, S = kGradStages;
   extern __shared__ __align__(16) unsigned char smem[];
-  pdlEnter();
+  waitForLaunchBefore();
   const int side = blockIdx.z / p.rank_passes, r0 = (blockIdx.z % p.rank_passes) * 16 * RT;
   const RowTile tile = findTile(p.seg, blockIdx.x);
   if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
@@ -981,7 +988,7 @@ template <typename T, bool SHARED>
 __global__ void __launch_bounds__(kJoinWarps * 32)
     lowRankJoinKernel(const int *__restrict__ slot_id, int slots, const float *__restrict__ p0,
                       const float *__restrict__ p1, T *g0, T *g1, long long elems0, long long elems1) {
-  pdlEnter();
+  waitForLaunchBefore();
   __shared__ float part[kJoinWarps][32];
   const int side = blockIdx.z, i = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long elems = side ? elems1 : elems0;

@@ -664,3 +664,134 @@ def test_beside_analog_tiles():
     # fp32 throughout: relative 2-norm errors of a few hundred roundings at most
     for got, want in [(y, y64), (h, h64)] + list(zip(grads, g64)):
         assert float((got.double() - want).norm()) <= 512 * F * float(want.norm())
+
+
+# ---- further calls that the documentation allows ---------------------------------------------------------------------
+
+
+def test_gradients_are_not_differentiable_again():
+    x = rand((6, 64), torch.float32, 1).requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    for y in (digital.layer_norm(x, w), digital.add_layer_norm(x, x * 2.0, w, p=0.1)[0], digital.dropout(x, 0.3)):
+        g, = torch.autograd.grad((y * y).sum(), [x], create_graph=True)
+        with pytest.raises(RuntimeError, match="not differentiable again"):
+            torch.autograd.grad(g.sum(), [x])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_low_rank_many_single_rows(dtype):
+    """Single rows of few adapters share tiles within a neighbourhood of 1024 requests; longer requests between them, empty
+    ones and rows without an adapter keep tiles of their own.  Each row's result is that of a call of its own."""
+    rng = np.random.default_rng(5)
+    lengths = rng.choice([0, 1, 1, 1, 1, 1, 1, 1, 2, 17], size=2300)
+    starts = np.concatenate([[3], 3 + np.cumsum(lengths)])
+    rows = int(starts[-1]) + 5
+    ids = rng.integers(-1, 3, size=2300)
+    per_row = np.full(rows, -1)
+    for j in range(2300):
+        per_row[starts[j]:starts[j + 1]] = ids[j]
+    per_row = torch.tensor(per_row, device="cuda")
+    x, base = rand((rows, 64), dtype, 1), rand((rows, 96), dtype, 2)
+    a, b = rand((3, 8, 64), dtype, 3, 0.125), rand((3, 8, 96), dtype, 4, 0.35)
+    scale = torch.tensor([0.5, 1.0, 2.0], device="cuda")
+    ids_t, starts_t = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in (ids, starts))
+    y64, off, _, _ = adapters_exact(x, base, a, b, scale, per_row)
+    y = digital.low_rank_add(base, x, a, b, scale, ids_t, starts_t)
+    within(y, y64, unit(dtype) * y64.abs() + off, "y")
+    assert torch.equal(y[per_row < 0], base[per_row < 0])
+    one = digital.low_rank_add(base, x, a, b, scale, per_row.int())  # each row a request
+    within(one, y64, unit(dtype) * y64.abs() + off, "one row each")
+    leaves = [t.requires_grad_() for t in (a, b)]
+    gy = rand((rows, 96), dtype, 9)
+    da, db = torch.autograd.grad(digital.low_rank_add(base, x, a, b, scale, ids_t, starts_t), leaves, gy)
+    for i in range(3):
+        m = per_row == i
+        u = float(scale[i]) * gy[m].double() @ b[i].detach().double().t()
+        v = float(scale[i]) * x[m].double() @ a[i].detach().double().t()
+        for got, l, r in ((da[i], u, x[m].double()), (db[i], v, gy[m].double())):
+            want = l.t() @ r
+            # two products and about 2300 sums in a row, 2^-17 of u or v at most beside them
+            bound = unit(dtype) * want.abs() + (l.abs().t() @ r.abs()) * (2400 * 2.0 ** -22)
+            within(got, want, bound, "gradient")
+
+
+def test_layer_norm_backward_of_the_c_interface_on_long_fp32_rows():
+    """fp32 callers of the C interface may hand over x and the residual as well as their sum."""
+    import ctypes as C
+
+    from aihwkit_b200 import _cabi
+
+    lib = _cabi.lib()
+    rows, p, seed, call = 5, 0.25, 3, 4
+    for cols in (768, 4096, 8192, 16384):
+        x, res, w, b = norm_case(rows, cols, torch.float32, True, p)
+        gy, gh = rand((rows, cols), torch.float32, 8), rand((rows, cols), torch.float32, 9)
+        leaves = [t.clone().requires_grad_() for t in (x, res, w, b)]
+        want = torch.autograd.grad(digital.add_layer_norm(*leaves, p=p, seed=seed, call=call), leaves, [gy, gh])
+        stats = torch.empty(2, rows, device="cuda")
+        y, h = torch.empty_like(x), torch.empty_like(x)
+        stream = torch.cuda.current_stream().cuda_stream
+        ptr = lambda t: t.data_ptr()
+        _cabi.check(lib.ab200_layer_norm_forward(ptr(x), cols, ptr(res), cols, ptr(w), ptr(b), ptr(y), cols, ptr(h), cols, ptr(stats),
+                                                 ptr(stats) + 4 * rows, rows, cols, 0, 0, 1e-5, p, seed, call, stream))
+        floats = C.c_longlong()
+        _cabi.check(lib.ab200_layer_norm_workspace(rows, cols, C.byref(floats)))
+        work = torch.empty(floats.value, device="cuda")
+        dh, dx, dw, db = torch.empty_like(x), torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+        _cabi.check(lib.ab200_layer_norm_backward(ptr(gy), cols, ptr(gh), cols, ptr(x), cols, ptr(res), cols, ptr(w), ptr(stats),
+                                                  ptr(stats) + 4 * rows, ptr(dh), cols, ptr(dx), cols, ptr(dw), ptr(db), ptr(work),
+                                                  rows, cols, 0, 0, p, seed, call, stream))
+        for got, ref in zip((dx, dh, dw, db), want):
+            assert torch.equal(got, ref)
+
+
+def test_two_calls_at_once_on_two_streams():
+    x, res, w, b = norm_case(3000, 1024, torch.bfloat16, True, 0.1)
+    c = adapters_case(3000, 6, 2, 768, 512, 8, torch.bfloat16, 5)
+    gy, ga = rand((3000, 1024), torch.bfloat16, 1), rand((3000, 512), torch.bfloat16, 2)
+
+    def norm():
+        leaves = [t.detach().requires_grad_() for t in (x, res, w, b)]
+        return torch.autograd.grad(digital.add_layer_norm(*leaves, p=0.1, seed=1, call=1)[0], leaves, gy)
+
+    def low_rank():
+        leaves = [c[0].detach().requires_grad_(), c[2].detach().requires_grad_(), c[3].detach().requires_grad_()]
+        return torch.autograd.grad(digital.low_rank_add(c[1], *leaves, *c[4:7]), leaves, ga)
+
+    want = norm() + low_rank()
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            n = norm()
+        with torch.cuda.stream(s2):
+            l = low_rank()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(n + l, want))
+
+
+def test_two_captured_graphs_replayed_in_turn():
+    """Workspaces belong to a call: two graphs of the same backward pass do not share them."""
+    c = adapters_case(600, 5, 2, 256, 320, 8, torch.float32, 5)
+    leaves = [t.requires_grad_() for t in (c[0], c[2], c[3])]
+    gys = [rand((600, 320), torch.float32, s) for s in (1, 2)]
+
+    def step(gy):
+        return torch.autograd.grad(digital.low_rank_add(c[1], *leaves, *c[4:7]), leaves, gy)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(gys[0])
+    side.synchronize()
+    graphs, outs = [], []
+    for gy in gys:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(gy))
+        graphs.append(g)
+    for _ in range(2):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for gy, out in zip(gys, outs):
+        assert all(torch.equal(p, q) for p, q in zip(out, step(gy)))
