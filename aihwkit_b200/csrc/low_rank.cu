@@ -100,28 +100,34 @@ __device__ __forceinline__ bool gatherRows(const Segments &s, RowTile &tile, int
   if (tile.rows == 1 && tile.id >= 0 && tile.alone) {
     const int first = tile.seg & ~1023, end = min(first + 1024, s.n);
     int before = 0, found = 0; // of the adapter's single rows: ahead of this one, all so far
-    for (int w = first; w < end && found - before < 16; w += 32) {
-      const int j = w + lane;
-      bool match = j < end && s.ids[j] == tile.id;
-      int row = j;
-      if (match && s.starts != nullptr) {
-        row = border(s, j + 1);
-        match = border(s, j + 2) == row + 1;
+    for (int w0 = first; w0 < end && found - before < 16; w0 += 256) {
+      int id[8], row[8], next[8]; // of 256 requests, all read before the first is looked at
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        const int j = w0 + q * 32 + lane;
+        id[q] = j < end ? s.ids[j] : -1;
+        row[q] = s.starts == nullptr ? j : j < end ? border(s, j + 1) : 0;
+        next[q] = s.starts == nullptr ? j + 1 : j < end ? border(s, j + 2) : 0;
       }
-      const unsigned hits = __ballot_sync(0xffffffffu, match);
-      if (tile.seg >= w) { // up to this row's own place
-        before += __popc(tile.seg < w + 32 ? hits & ((1u << (tile.seg - w)) - 1u) : hits);
-        if (tile.seg < w + 32 && before % 16 != 0) {
-          return false;
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        const int w = w0 + q * 32;
+        const bool match = id[q] == tile.id && next[q] == row[q] + 1;
+        const unsigned hits = __ballot_sync(0xffffffffu, match);
+        if (tile.seg >= w) { // up to this row's own place
+          before += __popc(tile.seg < w + 32 ? hits & ((1u << (tile.seg - w)) - 1u) : hits);
+          if (tile.seg < w + 32 && before % 16 != 0) {
+            return false;
+          }
         }
-      }
-      if (tile.seg < w + 32) {
-        const int at = found + __popc(hits & ((1u << lane) - 1u)) - before;
-        if (match && at >= 0 && at < 16) {
-          list[at] = row;
+        if (tile.seg < w + 32) {
+          const int at = found + __popc(hits & ((1u << lane) - 1u)) - before;
+          if (match && at >= 0 && at < 16) {
+            list[at] = row[q];
+          }
         }
+        found += __popc(hits);
       }
-      found += __popc(hits);
     }
     tile.rows = min(found - before, 16);
     __syncwarp();
