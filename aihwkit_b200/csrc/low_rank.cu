@@ -526,6 +526,9 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   // While x and a go through, the four 16-byte pieces of a row change places with the row, so that the eight
   // rows of a matrix lie in different banks
   const uint32_t own_x = g * 64 + (t ^ ((g >> 1) & 3)) * 16;
+  // and the pieces of b theirs in pairs of rows, for the four rows that a thread's neighbours read with it
+  const uint32_t own_b = Shape::XB + g * 64 + (t ^ (g & 2)) * 16;
+  const uint32_t read_b = Shape::XB + t * 64 + ((g >> 1) ^ (t & 2)) * 16 + (g & 1) * 8;
   // matrices of x (rows 0-7 and 8-15 of a fragment, two pieces) and of a (eight rows, four pieces)
   const uint32_t mat_row = lane & 15, mat_x = mat_row * 64, mat_swz = (mat_row >> 1) & 3, mat_f = (lane & 7) * 64;
 
@@ -537,12 +540,12 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   const auto fetchUnit = [&]() {
     if (f_unit < u_end) {
       const int c0 = f_unit * KS, col = c0 + t * E;
-      const uint32_t dst = ring + f_stage * Shape::STAGE + own;
+      const uint32_t dst = ring + f_stage * Shape::STAGE;
       const bool last = f_rank + RC >= p.rank;
       if (p.base != nullptr && last) {
-        fetchRows<T, VEC, 2 * MT, 512, 8>(dst, base_at + c0, base_8, col, p.n, g, rows_in);
+        fetchRows<T, VEC, 2 * MT, 512, 8>(dst + own, base_at + c0, base_8, col, p.n, g, rows_in);
       }
-      fetchRows<T, VEC, NT, 512, 8>(dst + Shape::XB, fb + (long long)(f_rank + g) * p.n + col, 8LL * p.n, col, p.n, f_rank + g,
+      fetchRows<T, VEC, NT, 512, 8>(dst + own_b, fb + (long long)(f_rank + g) * p.n + col, 8LL * p.n, col, p.n, f_rank + g,
                                     p.rank);
       f_rank = last ? 0 : f_rank + RC;
       f_unit += last ? W : 0;
@@ -731,7 +734,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
       uint4 b[RS / 4];
 #pragma unroll
       for (int q = 0; q < RS / 4; q++) {
-        b[q] = r + q * 4 < RC ? shared8B(src + Shape::XB + (r + q * 4 + t) * 64 + g * 8) : make_uint4(0, 0, 0, 0);
+        b[q] = r + q * 4 < RC ? shared8B(src + read_b + (r + q * 4) * 64) : make_uint4(0, 0, 0, 0);
       }
       if constexpr (kPairs<T>) {
         mmaPairs<decltype(first)::value>(acc, hi, lo, b);
@@ -892,7 +895,8 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
       const uint32_t dst = ring + stage * Shape::STAGE;
       const int row0 = i * kGradRows, rows = tile.rows - row0;
       const int col = unit * UC + (lane & 7) * E;
-      const uint32_t mine = dst + warp * Shape::XB + (lane >> 3) * 128 + (lane & 7) * 16;
+      // pieces change places with the row, so that four rows of a fragment lie in different banks
+      const uint32_t mine = dst + warp * Shape::XB + (lane >> 3) * 128 + ((lane & 7) ^ (2 * (lane >> 3))) * 16;
       fetchRows<T, VEC, kGradRows / 4, 512, 4>(mine, x + (row0 + (lane >> 3)) * ld + col, 4 * ld, col, width, lane >> 3, rows);
       if (u_wide) {
         for (int e = threadIdx.x; e < kGradRows * 4 * RT; e += kGradWarps * 32) {
@@ -930,7 +934,7 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
     fetch(i + S - 1, (i + S - 1) % S);
     const unsigned char *src = smem + (i % S) * Shape::STAGE;
     const float *us = reinterpret_cast<const float *>(src + kGradWarps * Shape::XB);
-    const unsigned char *xs = src + warp * Shape::XB + t * 128 + g * 16;
+    const unsigned char *xs = src + warp * Shape::XB + t * 128 + (g ^ (2 * t)) * 16;
     const float *uf = us + t * Shape::US + g;
     if constexpr (kPairs<T>) {
 #pragma unroll
@@ -974,11 +978,21 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const int r = i * 16 + h * 8 + g;
-      if (r < ranks) {
+      float *at = out + (long long)r * width + col;
+      if (r < ranks && VEC) {
+#pragma unroll
+        for (int j = 0; j < 2 * NJ; j += 4) {
+          if (col + j < width) {
+            *reinterpret_cast<float4 *>(at + j) =
+                make_float4(acc[i][j % NJ][2 * h + j / NJ], acc[i][j % NJ + 1][2 * h + j / NJ],
+                            acc[i][j % NJ + 2][2 * h + j / NJ], acc[i][j % NJ + 3][2 * h + j / NJ]);
+          }
+        }
+      } else if (r < ranks) {
 #pragma unroll
         for (int j = 0; j < 2 * NJ; j++) {
           if (col + j < width) {
-            out[(long long)r * width + col + j] = acc[i][j % NJ][2 * h + j / NJ];
+            at[j] = acc[i][j % NJ][2 * h + j / NJ];
           }
         }
       }
