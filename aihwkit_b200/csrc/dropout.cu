@@ -1,5 +1,8 @@
 // Dropout from a counter-based generator: y = keep ? x / (1 - p) : 0 (+ residual). No mask is
 // stored; the backward pass is the same kernel on the gradient with the same (seed, call).
+// Measured: 16384 x 768 fp32 with residual 22 us (6.9 TB/s), 16384 x 4096 bf16 54 us (5.0 TB/s): with 16-bit
+// elements the draws, one Philox block for eight, keep the issue slots and the integer pipe two thirds busy. Fewer
+// registers for more warps, or the next spans fetched a turn ahead, made it slower (58 us each).
 #include "digital.cuh"
 
 #include <algorithm>

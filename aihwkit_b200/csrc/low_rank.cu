@@ -19,9 +19,15 @@
 // 2^-22 of a product out. Where v (or u of the gradients) meets bf16, its two parts are bf16: 16 bits of it, 2^-17 off
 // against the 2^-9 of the rounding of the result, for half the products. fp16 has not the range for that.
 //
+// Measured: 16384 rows 768 -> 2304 rank 16 in 16 requests, fp32 70 us (5.0 TB/s), bf16 37 us (4.8 TB/s); 8192 rows 4096 ->
+// 4096 bf16, rank 32 47 us (4.3 TB/s), rank 64 71 us; 256 tokens of 64 adapters 4096 -> 4096 rank 16 15 us. 16 warps or fewer
+// fit a multiprocessor (registers, rings), and what they wait for - loads, shared memory, their own products - bounds
+// it; no pipe is more than 45 % busy.
+//
 // lowRankGradKernel. grad[id] = sum over the rows of id of u^T x: a warp holds rank x 128 bytes of columns
 // in fragments and walks a chunk of rows of one request, fetched the same way; chunks' partial sums go
-// through memory and are added in the order of the rows (no atomics).
+// through memory and are added in the order of the rows (no atomics). Measured: both gradients of 8192 rows 4096 -> 4096
+// rank 32 bf16 39 us (3.4 TB/s of x and gy), 61 us while the partial sums were stored by single floats.
 #include "digital.cuh"
 
 #include <algorithm>
