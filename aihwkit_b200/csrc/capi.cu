@@ -1080,6 +1080,20 @@ void digitalPointer(const char *what, const char *name, const void *p, long long
     AB200_FATAL(what << ": " << name << " is null");
   }
 }
+// distances between rows: not negative, and of outputs at least a row
+void digitalStrides(const char *what, long long rows, std::initializer_list<long long> inputs,
+                    std::initializer_list<std::pair<long long, int>> outputs) {
+  for (long long ld : inputs) {
+    if (ld < 0) {
+      AB200_FATAL(what << ": row strides must not be negative");
+    }
+  }
+  for (const auto &q : outputs) {
+    if (q.first < 0 || (rows > 1 && q.first < q.second)) {
+      AB200_FATAL(what << ": an output's row stride must be at least its row");
+    }
+  }
+}
 void digitalAdapters(const char *what, long long rows, int segments, const void *starts, const void *ids, int rank,
                      int adapters, int dtype) {
   digitalType(what, dtype);
@@ -1108,6 +1122,7 @@ int ab200_dropout(const void *x, long long x_stride, const void *residual, long 
   digitalRows("dropout", rows, cols, 1 << 30);
   digitalPointer("dropout", "x", x, rows);
   digitalPointer("dropout", "y", y, rows);
+  digitalStrides("dropout", rows, {x_stride, residual_stride}, {{y_stride, cols}});
   ab200::dropoutApply({x, x_stride}, {residual, residual_stride}, {y, y_stride}, rows, cols, dtype,
                       digitalDrop("dropout", p, seed, call), (cudaStream_t)stream);
   AB200_CATCH
@@ -1126,6 +1141,7 @@ int ab200_layer_norm_forward(const void *x, long long x_stride, const void *resi
   if ((mean == nullptr) != (rstd == nullptr)) {
     AB200_FATAL("layer_norm: mean and rstd are wanted together or not at all");
   }
+  digitalStrides("layer_norm", rows, {x_stride, residual_stride}, {{y_stride, cols}, {h ? h_stride : cols, cols}});
   ab200::NormArgs a = {{x, x_stride}, {residual, residual_stride}, {y, y_stride}, {h, h_stride}, weight, bias, mean,
                        rstd, rows, cols, dtype, param_dtype, eps, digitalDrop("layer_norm", p, seed, call)};
   ab200::normForward(a, (cudaStream_t)stream);
@@ -1153,6 +1169,8 @@ int ab200_layer_norm_backward(const void *gy, long long gy_stride, const void *g
   digitalPointer("layer_norm", "x", x, rows);
   digitalPointer("layer_norm", "mean", mean, rows);
   digitalPointer("layer_norm", "rstd", rstd, rows);
+  digitalStrides("layer_norm", rows, {gy_stride, gh_stride, x_stride, residual_stride},
+                 {{dh ? dh_stride : cols, cols}, {dx ? dx_stride : cols, cols}});
   const bool params = dweight != nullptr || dbias != nullptr;
   if (params) {
     digitalPointer("layer_norm", "workspace", workspace, rows);
@@ -1181,6 +1199,7 @@ int ab200_low_rank_apply(const void *x, long long x_stride, const void *base, lo
   if (y != nullptr) {
     digitalPointer("low_rank", "b", b, rows);
   }
+  digitalStrides("low_rank", rows, {x_stride, base_stride}, {{y ? y_stride : n, n}});
   if (y != nullptr && y == base && y_stride != base_stride) {
     AB200_FATAL("low_rank: y in the place of base needs base's row stride");
   }
@@ -1218,6 +1237,7 @@ int ab200_low_rank_grad(const void *x, long long x_stride, const float *u, void 
     digitalPointer("low_rank_grad", "gy", gy, rows);
     digitalPointer("low_rank_grad", "v", v, rows);
   }
+  digitalStrides("low_rank_grad", rows, {x_stride, gy_stride}, {});
   digitalPointer("low_rank_grad", "workspace", workspace, rows);
   ab200::LowRankGradArgs args = {{row_starts, adapter_ids, n_requests, rows}, {{x, x_stride}, {gy, gy_stride}}, {u, v},
                                  {da, db}, {k, n}, workspace, rank, n_adapters, dtype};

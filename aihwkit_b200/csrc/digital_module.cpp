@@ -509,6 +509,9 @@ Tensor lowRankAdd(const Tensor &base, const Tensor &x, const Tensor &a, const Te
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor y = out.defined() ? out : at::empty(base.sizes(), base.options());
   lowRankCompute(base, x, a, b, scale, ids, starts, y, Tensor());
+  if (out.defined() && !out.is_inference()) {
+    torch::autograd::impl::bump_version(out); // as torch's own in-place operations do, for who saved it
+  }
   return y;
 }
 

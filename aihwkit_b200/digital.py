@@ -76,7 +76,8 @@ def low_rank_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     ``row_starts[j + 1]`` (int32 on the device, one more value than requests, not decreasing); without ``row_starts`` request
     ``j`` is row ``j``.  Rows without an adapter, or in no request, are ``base``.  ``out`` takes the result - ``base`` itself
     among others, whose rows without an adapter are then not touched - in calls without gradients.  Differentiable in
-    ``base``, ``x``, ``a`` and ``b``.  Neighbouring rows of one adapter cost least as one request."""
+    ``base``, ``x``, ``a`` and ``b``.  Neighbouring rows of one adapter cost least as one request: in the backward pass above
+    all, where every request takes ``rank * (k + n)`` floats of workspace."""
     return _ext.low_rank_add(base, x, a, b, scale, adapter_ids, row_starts, out)
 
 

@@ -792,7 +792,8 @@ int ab200_mvm_forward_noalloc(const ab200_io_params *forward_io, const float *w_
  * model on analog tiles is adapted digitally: by low-rank adapters beside the tiles, with layer norms and
  * dropout around them. All pointers are device memory of the CURRENT device, `stream` one of its streams.
  * Matrices are rows of neighbouring elements, a row's start `*_stride` elements behind the one before
- * (a stride of 0 repeats one row and is for inputs only). Nothing is allocated and nothing is waited
+ * (a stride of 0 repeats one row and is for inputs only). Infinities and NaN make the results not finite that
+ * are summed from them, and no others. Nothing is allocated and nothing is waited
  * for; the calls can be captured into a graph. Sums, means and saved values are fp32 whatever the type,
  * results are rounded once. Outputs must not overlap inputs unless a call says so. */
 enum ab200_dtype { AB200_DTYPE_F32 = 0, AB200_DTYPE_F16 = 1, AB200_DTYPE_BF16 = 2 };
@@ -842,7 +843,7 @@ int ab200_layer_norm_backward(const void *gy, long long gy_stride, const void *g
  * The gradient of x is the same call on gy with a and b (k and n) exchanged, its v what the
  * gradient of a needs (u below).
  * grad: da = sum over an adapter's rows of u^T x, db = sum of v^T gy, of the type of x and gy, zero for
- * adapters without rows; each may be null. workspace has the bytes that ab200_low_rank_grad_workspace
+ * adapters without rows; each may be null. The workspace has rank * (k + n) floats for every request at least. workspace has the bytes that ab200_low_rank_grad_workspace
  * gives for the same sizes (k or n 0 where that gradient is not wanted; one_row_each: row_starts is null).
  * Requests may share an adapter; sums over rows are added in the order of the rows. Rows of one adapter
  * cost least as one request: each request has tiles of its own. */

@@ -54,7 +54,8 @@ def grad_args(**kw):
 @pytest.mark.parametrize("kw, match", [
     (dict(dtype=3), "unknown element type"), (dict(rows=-1), "number of rows"), (dict(rows=1 << 31), "number of rows"),
     (dict(cols=0), "1 to"), (dict(x=None), "x is null"), (dict(y=None), "y is null"), (dict(p=-0.1), "probability"),
-    (dict(p=1.5), "probability"), (dict(p=float("nan")), "probability")])
+    (dict(p=1.5), "probability"), (dict(p=float("nan")), "probability"), (dict(xs=-8), "strides"), (dict(rs=-1), "strides"),
+    (dict(rows=2, ys=7), "at least its row"), (dict(rows=2, ys=0), "at least its row")])
 def test_dropout_refuses(kw, match):
     refused("ab200_dropout", dropout_args(**kw), match)
 
@@ -62,7 +63,8 @@ def test_dropout_refuses(kw, match):
 @pytest.mark.parametrize("kw, match", [
     (dict(dtype=-1), "unknown element type"), (dict(pdtype=7), "unknown element type"), (dict(cols=16385), "1 to 16384"),
     (dict(cols=0), "1 to 16384"), (dict(rows=-1), "number of rows"), (dict(x=None), "x is null"), (dict(y=None), "y is null"),
-    (dict(mean=P), "together"), (dict(p=2.0), "probability")])
+    (dict(mean=P), "together"), (dict(p=2.0), "probability"), (dict(xs=-1), "strides"), (dict(rows=3, ys=4), "at least its row"),
+    (dict(rows=3, h=P, hs=4), "at least its row")])
 def test_layer_norm_refuses(kw, match):
     refused("ab200_layer_norm_forward", norm_args(**kw), match)
 
@@ -70,7 +72,7 @@ def test_layer_norm_refuses(kw, match):
 @pytest.mark.parametrize("kw, match", [
     (dict(gy=None), "gy is null"), (dict(x=None), "x is null"), (dict(mean=None), "mean is null"),
     (dict(rstd=None), "rstd is null"), (dict(dw=P), "workspace is null"), (dict(cols=20000), "1 to 16384"),
-    (dict(dtype=9), "unknown element type")])
+    (dict(dtype=9), "unknown element type"), (dict(gs=-8), "strides"), (dict(rows=2, dhs=1), "at least its row")])
 def test_layer_norm_backward_refuses(kw, match):
     refused("ab200_layer_norm_backward", norm_grad_args(**kw), match)
 
@@ -80,7 +82,8 @@ def test_layer_norm_backward_refuses(kw, match):
     (dict(ids=None), "adapter_ids is null"), (dict(rank=0), "rank"), (dict(rank=257), "rank"), (dict(adapters=0), "adapters"),
     (dict(adapters=70000), "adapters"), (dict(k=0), "elements"), (dict(n=0), "elements"), (dict(x=None), "x is null"),
     (dict(a=None), "a is null"), (dict(b=None), "b is null"), (dict(scale=None), "scale is null"), (dict(y=None), "neither"),
-    (dict(base=P, bs=16), "row stride"), (dict(rows=-1, n_req=-1), "number of")])
+    (dict(base=P, bs=16), "row stride"), (dict(xs=-1), "strides"),
+    (dict(rows=2, n_req=2, ys=7), "at least its row"), (dict(rows=-1, n_req=-1), "number of")])
 def test_low_rank_refuses(kw, match):
     refused("ab200_low_rank_apply", low_rank_args(**kw), match)
 
@@ -88,7 +91,7 @@ def test_low_rank_refuses(kw, match):
 @pytest.mark.parametrize("kw, match", [
     (dict(dtype=3), "unknown element type"), (dict(rank=300), "rank"), (dict(k=0), "elements"), (dict(gy=None), "gy is null"),
     (dict(u=None), "u is null"), (dict(v=None), "v is null"), (dict(work=None), "workspace is null"),
-    (dict(n_req=3), "one request per row")])
+    (dict(n_req=3), "one request per row"), (dict(gs=-2), "strides")])
 def test_low_rank_grad_refuses(kw, match):
     refused("ab200_low_rank_grad", grad_args(**kw), match)
 

@@ -795,3 +795,36 @@ def test_two_captured_graphs_replayed_in_turn():
     torch.cuda.synchronize()
     for gy, out in zip(gys, outs):
         assert all(torch.equal(p, q) for p, q in zip(out, step(gy)))
+
+
+def test_in_place_results_are_seen_by_autograd():
+    """A result written over a tensor that autograd has saved is found out, as with torch's own in-place operations."""
+    x, base, a, b, scale, ids, starts, _ = adapters_case(40, 4, 2, 64, 96, 8, torch.float32, 3)
+    w = torch.ones(96, device="cuda", requires_grad=True)
+    y = base * w  # keeps base for the gradient of w
+    with torch.no_grad():
+        digital.low_rank_add(base, x, a, b, scale, ids, starts, out=base)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_non_finite_rows_stay_to_themselves():
+    """Infinities and NaN in rows with an adapter make those rows not finite, and no row beside them in a tile."""
+    for dtype in TYPES:
+        for requests, ragged in ((40, False), (2, True)):
+            x, base, a, b, scale, ids, starts, per_row = adapters_case(40, requests, 2, 64, 96, 8, dtype, 3, ragged)
+            want = digital.low_rank_add(base, x, a, b, scale, ids, starts)
+            used = (per_row >= 0).nonzero().flatten()
+            bad = used[::3]
+            x2 = x.clone()
+            x2[bad[::2], 5], x2[bad[1::2], 7] = float("nan"), float("inf")
+            got = digital.low_rank_add(base, x2, a, b, scale, ids, starts)
+            good = torch.ones(40, dtype=torch.bool, device="cuda")
+            good[bad] = False
+            assert torch.equal(got[good], want[good]) and not torch.isfinite(got[bad]).any()
+    x, res, w, b = norm_case(9, 300, torch.bfloat16, True, 0.0)
+    y, h = digital.add_layer_norm(x, res, w, b)
+    res[4, 17] = float("inf")
+    y2, h2 = digital.add_layer_norm(x, res, w, b)
+    keep = torch.arange(9, device="cuda") != 4
+    assert torch.equal(y2[keep], y[keep]) and torch.isnan(y2[4]).all()
