@@ -347,43 +347,45 @@ __device__ __forceinline__ void mmaPairs(float (&acc)[MT][NJ][4], const uint32_t
 
 // ---- rings of cp.async ------------------------------------------------------------------------
 // 16 bytes of a row to shared memory, from `src`, the place of column `col`; columns past the end, and all
-// of them where `in` is false, become zeros without a read (nor a branch). fp32 rows that 16-byte
-// accesses do not fit go by elements, 16-bit ones through registers (fetchRows).
-template <typename T, bool VEC>
+// of them where `in` is false, become zeros without a read (nor a branch)
+template <typename T>
 __device__ __forceinline__ void fetch16B(uint32_t dst, const T *src, int col, int cols, bool in) {
-  if (VEC) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in && col < cols ? 16 : 0)
-                 : "memory");
-  } else {
-    static_assert(VEC || sizeof(T) == 4, "16-bit elements are below what cp.async copies");
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * i), "l"(src + i),
-                   "r"(in && col + i < cols ? 4 : 0)
-                   : "memory");
-    }
-  }
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in && col < cols ? 16 : 0)
+               : "memory");
 }
 // N such pieces, of rows `step` elements apart and STRIDE bytes apart in shared memory, of which the first
-// `rows` are there in steps of EVERY from row `first`; what goes through registers is read before any of it is stored
-template <typename T, bool VEC, int N, int STRIDE, int EVERY>
+// `rows` are there in steps of EVERY from row `first`
+template <typename T, int N, int STRIDE, int EVERY>
 __device__ __forceinline__ void fetchRows(uint32_t dst, const T *src, long long step, int col, int cols, int first, int rows) {
-  if constexpr (VEC || sizeof(T) == 4) {
 #pragma unroll
-    for (int q = 0; q < N; q++, src += step) {
-      fetch16B<T, VEC>(dst + q * STRIDE, src, col, cols, q * EVERY + first < rows);
-    }
-  } else {
-    uint4 piece[N];
+  for (int q = 0; q < N; q++, src += step) {
+    fetch16B(dst + q * STRIDE, src, col, cols, q * EVERY + first < rows);
+  }
+}
+// Rows that 16-byte accesses do not fit: N rows of PIECES pieces of 16 bytes from column c0 on, element by element
+// with neighbouring lanes on neighbouring elements (a lane that went for its own 16 bytes touched 32 sectors with
+// every load: 8192 rows of 2001 -> 2047 rank 16 bf16 took 116 us). fp32 goes by cp.async; 16-bit elements, below what
+// it copies, through registers. rowOf gives a row's first element; place(row, piece) is where a piece goes among its row's.
+template <typename T, int N, int PIECES, typename RowOf, typename Place>
+__device__ __forceinline__ void fetchOdd(unsigned char *dst, int lane, int c0, int cols, int rows, RowOf rowOf, Place place) {
+  constexpr int E = 16 / sizeof(T), PER_ROW = PIECES * E; // elements of a row
+  constexpr int ROWS = PER_ROW >= 32 ? 1 : 32 / PER_ROW, PARTS = PER_ROW >= 32 ? PER_ROW / 32 : 1;
 #pragma unroll
-    for (int q = 0; q < N; q++, src += step) {
-      piece[q] = load16B<T, false>(src - col, col, q * EVERY + first < rows ? cols : 0);
-    }
+  for (int i = 0; i < N / ROWS; i++) {
+    const int r = i * ROWS + lane / (32 / ROWS);
+    const T *row = rowOf(r);
 #pragma unroll
-    for (int q = 0; q < N; q++) {
-      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + q * STRIDE), "r"(piece[q].x), "r"(piece[q].y),
-                   "r"(piece[q].z), "r"(piece[q].w)
-                   : "memory");
+    for (int h = 0; h < PARTS; h++) {
+      const int e = h * 32 + lane % (32 / ROWS);
+      const bool in = r < rows && c0 + e < cols;
+      unsigned char *at = dst + r * PIECES * 16 + place(r, e / E) * 16 + e % E * (int)sizeof(T);
+      if constexpr (sizeof(T) == 4) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(at)),
+                     "l"(row + c0 + e), "r"(in ? 4 : 0)
+                     : "memory");
+      } else {
+        *reinterpret_cast<uint16_t *>(at) = in ? reinterpret_cast<const uint16_t *>(row)[c0 + e] : (uint16_t)0;
+      }
     }
   }
 }
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
     return;
   }
   const int r_pad = (p.rank + 7) & ~7, vs = r_pad + 4;
-  const unsigned char *held = smem + warp * S * Shape::STAGE; // this warp's ring, as it is read
+  unsigned char *held = smem + warp * S * Shape::STAGE; // this warp's ring
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(held);
   // v of the tile as the second product's operands: [fragment][8 ranks (bf16: 16)][hi, lo][lane][4]
   float *v = reinterpret_cast<float *>(smem + Shape::RING);
@@ -538,6 +540,9 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   // matrices of x (rows 0-7 and 8-15 of a fragment, two pieces) and of a (eight rows, four pieces)
   const uint32_t mat_row = lane & 15, mat_x = mat_row * 64, mat_swz = (mat_row >> 1) & 3, mat_f = (lane & 7) * 64;
 
+  // row r of the tile against row0, for accesses whose rows are not the thread's own
+  const auto rowAt = [&](int r) { return MT == 1 ? (long long)(tile_rows[warp][r] - tile.row0) : (long long)r; };
+
   // v = x a^T: steps of KS along k are dealt to the blocks of the cluster and to the warps in turn
   const int steps = (p.k + KS - 1) / KS, steps_per = (steps + p.cluster - 1) / p.cluster;
   const int s_begin = part * steps_per + warp, s_end = min(steps, part * steps_per + steps_per);
@@ -546,13 +551,23 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   const auto fetchUnit = [&]() {
     if (f_unit < u_end) {
       const int c0 = f_unit * KS, col = c0 + t * E;
-      const uint32_t dst = ring + f_stage * Shape::STAGE;
       const bool last = f_rank + RC >= p.rank;
-      if (p.base != nullptr && last) {
-        fetchRows<T, VEC, 2 * MT, 512, 8>(dst + own, base_at + c0, base_8, col, p.n, g, rows_in);
+      const bool with_base = p.base != nullptr && last;
+      if constexpr (VEC) {
+        const uint32_t dst = ring + f_stage * Shape::STAGE;
+        if (with_base) {
+          fetchRows<T, 2 * MT, 512, 8>(dst + own, base_at + c0, base_8, col, p.n, g, rows_in);
+        }
+        fetchRows<T, NT, 512, 8>(dst + own_b, fb + (long long)(f_rank + g) * p.n + col, 8LL * p.n, col, p.n, f_rank + g, p.rank);
+      } else {
+        unsigned char *dst = held + f_stage * Shape::STAGE;
+        if (with_base) {
+          fetchOdd<T, TM, 4>(dst, lane, c0, p.n, rows_in, [&](int r) { return base + rowAt(r) * p.base_ld; },
+                             [](int, int piece) { return piece; });
+        }
+        fetchOdd<T, RC, 4>(dst + Shape::XB, lane, c0, p.n, p.rank - f_rank, [&](int r) { return fb + (long long)(f_rank + r) * p.n; },
+                           [](int r, int piece) { return piece ^ (r & 2); });
       }
-      fetchRows<T, VEC, NT, 512, 8>(dst + own_b, fb + (long long)(f_rank + g) * p.n + col, 8LL * p.n, col, p.n, f_rank + g,
-                                    p.rank);
       f_rank = last ? 0 : f_rank + RC;
       f_unit += last ? W : 0;
     }
@@ -571,9 +586,17 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
     const auto fetchStep = [&](int s, int stage) {
       if (s < s_end) {
         const int c0 = s * KS, k0 = c0 + t * E;
-        const uint32_t dst = ring + stage * Shape::STAGE + own_x;
-        fetchRows<T, VEC, 2 * MT, 512, 8>(dst, x_at + c0, x_8, k0, p.k, g, rows_in);
-        fetchRows<T, VEC, NT, 512, 8>(dst + Shape::XB, fa + (long long)(r0 + g) * p.k + k0, 8LL * p.k, k0, p.k, r0 + g, p.rank);
+        if constexpr (VEC) {
+          const uint32_t dst = ring + stage * Shape::STAGE + own_x;
+          fetchRows<T, 2 * MT, 512, 8>(dst, x_at + c0, x_8, k0, p.k, g, rows_in);
+          fetchRows<T, NT, 512, 8>(dst + Shape::XB, fa + (long long)(r0 + g) * p.k + k0, 8LL * p.k, k0, p.k, r0 + g, p.rank);
+        } else {
+          unsigned char *dst = held + stage * Shape::STAGE;
+          const auto swizzled = [](int r, int piece) { return piece ^ ((r >> 1) & 3); };
+          fetchOdd<T, TM, 4>(dst, lane, c0, p.k, rows_in, [&](int r) { return x + rowAt(r) * p.x_ld; }, swizzled);
+          fetchOdd<T, RC, 4>(dst + Shape::XB, lane, c0, p.k, p.rank - r0, [&](int r) { return fa + (long long)(r0 + r) * p.k; },
+                             swizzled);
+        }
       }
       fetchCommit();
     };
@@ -711,7 +734,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   if (p.y == nullptr) {
     return;
   }
-  if (p.base == nullptr) { // zeros in its place, in every stage (each thread reads its own)
+  if (VEC && p.base == nullptr) { // zeros in its place, in every stage (each thread reads its own)
     for (int q = 0; q < S * 2 * MT; q++) {
       *reinterpret_cast<uint4 *>(smem + warp * S * Shape::STAGE + q / (2 * MT) * Shape::STAGE + own + q % (2 * MT) * 512) =
           make_uint4(0, 0, 0, 0);
@@ -725,7 +748,8 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
     fetchUnit();
     fetchWait<S - 1>();
     __syncwarp(); // b is read by other lanes than fetched it
-    const unsigned char *src = held + stage * Shape::STAGE;
+    unsigned char *held_now = held + stage * Shape::STAGE;
+    const unsigned char *src = held_now;
     stage = stage + 1 == S ? 0 : stage + 1;
     constexpr int RS = kPairs<T> ? 16 : 8; // ranks to a product
     const auto ranks = [&](int r, auto first) {
@@ -768,19 +792,31 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
 #pragma unroll
     for (int q = 0; q < 2 * MT; q++, dst += y_8) {
       if (q * 8 + g < rows_in) {
-        const uint4 old = shared16B(src + own + q * 512);
+        const uint4 old = VEC || p.base != nullptr ? shared16B(src + own + q * 512) : make_uint4(0, 0, 0, 0);
         float o[E];
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
           o[j] = acc[q / 2][j][2 * (q % 2)] + elemOf<T>(old, j);
           o[NJ + j] = acc[q / 2][j][2 * (q % 2) + 1] + elemOf<T>(old, NJ + j);
         }
-        if (VEC) {
+        if constexpr (VEC) {
           if (col < p.n) {
             store16B<T, true>(dst, 0, E, o);
           }
         } else {
-          store16B<T, false>(dst - col, col, p.n, o);
+          store16B<T, true>(reinterpret_cast<T *>(held_now + own + q * 512), 0, E, o);
+        }
+      }
+    }
+    if constexpr (!VEC) {
+      // the unit's results are in base's place: out by rows, neighbouring lanes on neighbouring elements
+      __syncwarp();
+      constexpr int ROWS = 32 / KS; // rows a turn
+      const int e = lane % KS;
+#pragma unroll 8
+      for (int r = lane / KS; r < rows_in; r += ROWS) {
+        if (u * KS + e < p.n) {
+          y[rowAt(r) * p.y_ld + u * KS + e] = reinterpret_cast<const T *>(held_now + r * 64)[e];
         }
       }
     }
@@ -827,7 +863,9 @@ void launchApply(Apply p, const LowRankRows &seg, int shift, cudaStream_t stream
 template <typename T, bool VEC> void dispatchApply(const Apply &p, const LowRankRows &seg, cudaStream_t st) {
   // Requests of 16 rows and fewer on average (decoding) take tiles of 16 rows, longer ones of 64, or 32 with
   // more than 16 ranks: with the fragments of 64 rows only three blocks fitted a multiprocessor (8192 rows,
-  // 4096 -> 4096, rank 32, bf16: 78 us, 51 with 32 rows)
+  // 4096 -> 4096, rank 32, bf16: 78 us, 51 with 32 rows). 32 rows, too, where 16-bit elements pass registers one by one,
+  // 64 of them at a time with the longer tile
+  constexpr int kLong = VEC || sizeof(T) == 4 ? 4 : 2, kLongShift = kLong == 4 ? 6 : 5;
   if (seg.starts == nullptr || seg.rows <= 16LL * seg.segments) {
     if (p.rank <= 8) {
       launchApply<T, VEC, 1, 1>(p, seg, 4, st);
@@ -839,9 +877,9 @@ template <typename T, bool VEC> void dispatchApply(const Apply &p, const LowRank
       launchApply<T, VEC, 1, 8>(p, seg, 4, st);
     }
   } else if (p.rank <= 8) {
-    launchApply<T, VEC, 4, 1>(p, seg, 6, st);
+    launchApply<T, VEC, kLong, 1>(p, seg, kLongShift, st);
   } else if (p.rank <= 16) {
-    launchApply<T, VEC, 4, 2>(p, seg, 6, st);
+    launchApply<T, VEC, kLong, 2>(p, seg, kLongShift, st);
   } else if (p.rank <= 32) {
     launchApply<T, VEC, 2, 4>(p, seg, 5, st);
   } else {
@@ -900,14 +938,19 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
     if (i < chunks) {
       const uint32_t dst = ring + stage * Shape::STAGE;
       const int row0 = i * kGradRows, rows = tile.rows - row0;
-      const int col = unit * UC + (lane & 7) * E;
       // pieces change places with the row, so that four rows of a fragment lie in different banks
-      const uint32_t mine = dst + warp * Shape::XB + (lane >> 3) * 128 + ((lane & 7) ^ (2 * (lane >> 3))) * 16;
-      fetchRows<T, VEC, kGradRows / 4, 512, 4>(mine, x + (row0 + (lane >> 3)) * ld + col, 4 * ld, col, width, lane >> 3, rows);
+      if constexpr (VEC) {
+        const int col = unit * UC + (lane & 7) * E;
+        const uint32_t mine = dst + warp * Shape::XB + (lane >> 3) * 128 + ((lane & 7) ^ (2 * (lane >> 3))) * 16;
+        fetchRows<T, kGradRows / 4, 512, 4>(mine, x + (row0 + (lane >> 3)) * ld + col, 4 * ld, col, width, lane >> 3, rows);
+      } else {
+        fetchOdd<T, kGradRows, 8>(smem + stage * Shape::STAGE + warp * Shape::XB, lane, unit * UC, width, rows,
+                                  [&](int r) { return x + (row0 + r) * ld; }, [](int r, int piece) { return piece ^ (2 * (r & 3)); });
+      }
       if (u_wide) {
         for (int e = threadIdx.x; e < kGradRows * 4 * RT; e += kGradWarps * 32) {
           const int r = e / (4 * RT), c = e % (4 * RT) * 4;
-          fetch16B<float, true>(dst + kGradWarps * Shape::XB + (r * Shape::US + c) * 4, u + (long long)(row0 + r) * p.rank + c,
+          fetch16B(dst + kGradWarps * Shape::XB + (r * Shape::US + c) * 4, u + (long long)(row0 + r) * p.rank + c,
                                 c, ranks, r < rows);
         }
       } else {
