@@ -365,28 +365,33 @@ __device__ __forceinline__ void fetchRows(uint32_t dst, const T *src, long long 
 // Rows that 16-byte accesses do not fit: N rows of PIECES pieces of 16 bytes from column c0 on, element by element
 // with neighbouring lanes on neighbouring elements (a lane that went for its own 16 bytes touched 32 sectors with
 // every load: 8192 rows of 2001 -> 2047 rank 16 bf16 took 116 us). fp32 goes by cp.async; 16-bit elements, below what
-// it copies, through registers. rowOf gives a row's first element; place(row, piece) is where a piece goes among its row's.
-template <typename T, int N, int PIECES, typename RowOf, typename Place>
-__device__ __forceinline__ void fetchOdd(unsigned char *dst, int lane, int c0, int cols, int rows, RowOf rowOf, Place place) {
+// it copies, through registers. rowOf gives a row's first element (the next row's is `step` further unless the rows
+// come from a LIST), place(row, piece) where a piece goes among its row's.
+template <typename T, int N, int PIECES, bool LIST, typename RowOf, typename Place>
+__device__ __forceinline__ void fetchOdd(unsigned char *dst, int lane, int c0, int cols, int rows, RowOf rowOf, long long step,
+                                         Place place) {
   constexpr int E = 16 / sizeof(T), PER_ROW = PIECES * E; // elements of a row
   constexpr int ROWS = PER_ROW >= 32 ? 1 : 32 / PER_ROW, PARTS = PER_ROW >= 32 ? PER_ROW / 32 : 1;
+  const int r0 = lane / (32 / ROWS), e0 = lane % (32 / ROWS);
+  const T *next = rowOf(r0) + c0 + e0;
 #pragma unroll
   for (int i = 0; i < N / ROWS; i++) {
-    const int r = i * ROWS + lane / (32 / ROWS);
-    const T *row = rowOf(r);
+    const int r = i * ROWS + r0;
+    const T *src = LIST ? rowOf(r) + c0 + e0 : next;
 #pragma unroll
     for (int h = 0; h < PARTS; h++) {
-      const int e = h * 32 + lane % (32 / ROWS);
+      const int e = h * 32 + e0;
       const bool in = r < rows && c0 + e < cols;
       unsigned char *at = dst + r * PIECES * 16 + place(r, e / E) * 16 + e % E * (int)sizeof(T);
       if constexpr (sizeof(T) == 4) {
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(at)),
-                     "l"(row + c0 + e), "r"(in ? 4 : 0)
+                     "l"(src + h * 32), "r"(in ? 4 : 0)
                      : "memory");
       } else {
-        *reinterpret_cast<uint16_t *>(at) = in ? reinterpret_cast<const uint16_t *>(row)[c0 + e] : (uint16_t)0;
+        *reinterpret_cast<uint16_t *>(at) = in ? reinterpret_cast<const uint16_t *>(src)[h * 32] : (uint16_t)0;
       }
     }
+    next += ROWS * step;
   }
 }
 __device__ __forceinline__ void fetchCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -562,11 +567,12 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
       } else {
         unsigned char *dst = held + f_stage * Shape::STAGE;
         if (with_base) {
-          fetchOdd<T, TM, 4>(dst, lane, c0, p.n, rows_in, [&](int r) { return base + rowAt(r) * p.base_ld; },
-                             [](int, int piece) { return piece; });
+          fetchOdd<T, TM, 4, MT == 1>(dst, lane, c0, p.n, rows_in, [&](int r) { return base + rowAt(r) * p.base_ld; }, p.base_ld,
+                                      [](int, int piece) { return piece; });
         }
-        fetchOdd<T, RC, 4>(dst + Shape::XB, lane, c0, p.n, p.rank - f_rank, [&](int r) { return fb + (long long)(f_rank + r) * p.n; },
-                           [](int r, int piece) { return piece ^ (r & 2); });
+        fetchOdd<T, RC, 4, false>(dst + Shape::XB, lane, c0, p.n, p.rank - f_rank,
+                                  [&](int r) { return fb + (long long)(f_rank + r) * p.n; }, p.n,
+                                  [](int r, int piece) { return piece ^ (r & 2); });
       }
       f_rank = last ? 0 : f_rank + RC;
       f_unit += last ? W : 0;
@@ -593,9 +599,9 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
         } else {
           unsigned char *dst = held + stage * Shape::STAGE;
           const auto swizzled = [](int r, int piece) { return piece ^ ((r >> 1) & 3); };
-          fetchOdd<T, TM, 4>(dst, lane, c0, p.k, rows_in, [&](int r) { return x + rowAt(r) * p.x_ld; }, swizzled);
-          fetchOdd<T, RC, 4>(dst + Shape::XB, lane, c0, p.k, p.rank - r0, [&](int r) { return fa + (long long)(r0 + r) * p.k; },
-                             swizzled);
+          fetchOdd<T, TM, 4, MT == 1>(dst, lane, c0, p.k, rows_in, [&](int r) { return x + rowAt(r) * p.x_ld; }, p.x_ld, swizzled);
+          fetchOdd<T, RC, 4, false>(dst + Shape::XB, lane, c0, p.k, p.rank - r0,
+                                    [&](int r) { return fa + (long long)(r0 + r) * p.k; }, p.k, swizzled);
         }
       }
       fetchCommit();
@@ -944,8 +950,9 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
         const uint32_t mine = dst + warp * Shape::XB + (lane >> 3) * 128 + ((lane & 7) ^ (2 * (lane >> 3))) * 16;
         fetchRows<T, kGradRows / 4, 512, 4>(mine, x + (row0 + (lane >> 3)) * ld + col, 4 * ld, col, width, lane >> 3, rows);
       } else {
-        fetchOdd<T, kGradRows, 8>(smem + stage * Shape::STAGE + warp * Shape::XB, lane, unit * UC, width, rows,
-                                  [&](int r) { return x + (row0 + r) * ld; }, [](int r, int piece) { return piece ^ (2 * (r & 3)); });
+        fetchOdd<T, kGradRows, 8, false>(smem + stage * Shape::STAGE + warp * Shape::XB, lane, unit * UC, width, rows,
+                                         [&](int r) { return x + (row0 + r) * ld; }, ld,
+                                         [](int r, int piece) { return piece ^ (2 * (r & 3)); });
       }
       if (u_wide) {
         for (int e = threadIdx.x; e < kGradRows * 4 * RT; e += kGradWarps * 32) {
