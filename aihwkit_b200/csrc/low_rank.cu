@@ -869,9 +869,9 @@ void launchApply(Apply p, const LowRankRows &seg, int shift, cudaStream_t stream
 template <typename T, bool VEC> void dispatchApply(const Apply &p, const LowRankRows &seg, cudaStream_t st) {
   // Requests of 16 rows and fewer on average (decoding) take tiles of 16 rows, longer ones of 64, or 32 with
   // more than 16 ranks: with the fragments of 64 rows only three blocks fitted a multiprocessor (8192 rows,
-  // 4096 -> 4096, rank 32, bf16: 78 us, 51 with 32 rows). 32 rows, too, where 16-bit elements pass registers one by one,
-  // 64 of them at a time with the longer tile
-  constexpr int kLong = VEC || sizeof(T) == 4 ? 4 : 2, kLongShift = kLong == 4 ? 6 : 5;
+  // 4096 -> 4096, rank 32, bf16: 78 us, 51 with 32 rows). 32 rows, too, where elements are fetched one by
+  // one (8192 x 2001 -> 2047 rank 16 fp32: 93 us with 64 rows, 71 with 32)
+  constexpr int kLong = VEC ? 4 : 2, kLongShift = kLong == 4 ? 6 : 5;
   if (seg.starts == nullptr || seg.rows <= 16LL * seg.segments) {
     if (p.rank <= 8) {
       launchApply<T, VEC, 1, 1>(p, seg, 4, st);
