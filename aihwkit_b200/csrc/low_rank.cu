@@ -16,8 +16,8 @@
 // through distributed shared memory in rank order, and each block takes a share of the columns.
 // Products: bf16 x bf16 and fp16 x fp16 are exact in the fp32 sum; fp32 factors (v, and x, a, b of
 // fp32 calls) are split into two TF32 parts, hi + lo, and multiplied as hi hi + lo hi + hi lo, which leaves
-// 2^-22 of a product out. Where v (or u of the gradients) meets bf16, its two parts are bf16: 16 bits of it, 2^-17 off
-// against the 2^-9 of the rounding of the result, for half the products. fp16 has not the range for that.
+// 2^-22 of a product out. Where v (or u of the gradients) meets bf16, its three parts are bf16 and hold all of its 24
+// bits, three products in place of the four that TF32 parts take at half the rate. fp16 has not the range for that.
 //
 // Measured: 16384 rows 768 -> 2304 rank 16 in 16 requests, fp32 70 us (5.0 TB/s), bf16 37 us (4.8 TB/s); 8192 rows 4096 ->
 // 4096 bf16, rank 32 47 us (4.3 TB/s), rank 64 71 us; 256 tokens of 64 adapters 4096 -> 4096 rank 16 15 us. 16 warps or fewer
@@ -192,13 +192,25 @@ __device__ __forceinline__ void split(float v, uint32_t &hi, uint32_t &lo) {
   lo = __float_as_uint(v - __uint_as_float(hi));
 }
 
-// a and b as the halves of a word, in bf16, and what is left of them in another
-__device__ __forceinline__ void splitPair(float a, float b, uint32_t &hi, uint32_t &lo) {
-  hi = pack2<__nv_bfloat16>(a, b);
-  const float2 f = unpack2<__nv_bfloat16>(hi);
-  lo = pack2<__nv_bfloat16>(a - f.x, b - f.y);
+// a and b as the halves of a word, in bf16, what is left of them (16 bits at most) in another, and what is left of
+// that (8 bits) in a third: fp32 = p[0] + p[1] + p[2]
+constexpr int kParts = 3;
+__device__ __forceinline__ void splitPair(float a, float b, uint32_t p[kParts]) {
+#pragma unroll
+  for (int q = 0; q < kParts; q++) {
+    p[q] = pack2<__nv_bfloat16>(a, b);
+    const float2 f = unpack2<__nv_bfloat16>(p[q]);
+    a -= f.x;
+    b -= f.y;
+  }
 }
 template <typename T> constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
+// bytes of an element of v as an operand of the second product, and the ranks that a product takes
+template <typename T> constexpr int kOperandBytes = kPairs<T> ? 2 * kParts : 8;
+template <typename T> constexpr int kOperandRanks = kPairs<T> ? 16 : 8;
+template <typename T> __host__ __device__ __forceinline__ int operandRanks(int rank) {
+  return (rank + kOperandRanks<T> - 1) / kOperandRanks<T> * kOperandRanks<T>;
+}
 
 // 16 bytes of a row: eight 16-bit or four fp32 neighbours; elements past the end read as zero
 template <typename T, bool VEC>
@@ -315,10 +327,9 @@ __device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], const uint32
 }
 
 // The same for bf16 and sixteen rows of the factor: rows t and t + 4 (b[0], b[1]) go as a pair, and rows t + 8 and
-// t + 12 (b[2], b[3]); hi and lo hold their factors in the same pairs
+// t + 12 (b[2], b[3]); the parts of their factors come in the same pairs
 template <bool FIRST, int MT, int NJ>
-__device__ __forceinline__ void mmaPairs(float (&acc)[MT][NJ][4], const uint32_t (&hi)[MT][4], const uint32_t (&lo)[MT][4],
-                                         const uint4 (&b)[4]) {
+__device__ __forceinline__ void mmaPairs(float (&acc)[MT][NJ][4], const uint32_t (&parts)[kParts][MT][4], const uint4 (&b)[4]) {
   uint32_t p[NJ][2];
 #pragma unroll
   for (int j = 0; j < NJ; j++) {
@@ -331,15 +342,15 @@ __device__ __forceinline__ void mmaPairs(float (&acc)[MT][NJ][4], const uint32_t
     }
   }
 #pragma unroll
-  for (int term = 0; term < 2; term++) {
+  for (int part = kParts - 1; part >= 0; part--) {
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
 #pragma unroll
       for (int i = 0; i < MT; i++) {
-        if (FIRST && term == 0) {
+        if (FIRST && part == kParts - 1) {
           acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
         }
-        mma16<__nv_bfloat16>(acc[i][j], term == 0 ? lo[i] : hi[i], p[j][0], p[j][1]);
+        mma16<__nv_bfloat16>(acc[i][j], parts[part][i], p[j][0], p[j][1]);
       }
     }
   }
@@ -452,9 +463,9 @@ template <int MT, int NT> struct ApplyShape {
   static constexpr int SHARES = MT == 1 ? W * TM * (RC + 4) * 4 : 0;
   // blocks to a multiprocessor, bounded by registers and shared memory
   static constexpr int BLOCKS = MT == 1 ? 2 : 4;
-  static size_t bytes(int rank) {
+  template <typename T> static size_t bytes(int rank) {
     const int vs = ((rank + 7) & ~7) + 4;
-    return RING + SHARES + (size_t)TM * ((vs - 4) * 8 + vs * 4);
+    return RING + SHARES + (size_t)TM * (operandRanks<T>(rank) * kOperandBytes<T> + vs * 4);
   }
 };
 
@@ -521,9 +532,10 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   const int r_pad = (p.rank + 7) & ~7, vs = r_pad + 4;
   unsigned char *held = smem + warp * S * Shape::STAGE; // this warp's ring
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(held);
-  // v of the tile as the second product's operands: [fragment][8 ranks (bf16: 16)][hi, lo][lane][4]
+  const int c_end = operandRanks<T>(p.rank);
+  // v of the tile as the second product's operands: [fragment][8 ranks (bf16: 16)][parts][lane][4]
   float *v = reinterpret_cast<float *>(smem + Shape::RING);
-  float *mine = v + TM * r_pad * 2; // [TM][vs]: this block's share of v
+  float *mine = v + TM * c_end * kOperandBytes<T> / 4; // [TM][vs]: this block's share of v
   float *shares = mine + TM * vs;   // [W][TM][RC + 4], of tiles of 16 rows
   const float scale = p.scale[tile.id];
   const T *fa = (const T *)p.a + (long long)tile.id * p.rank * p.k;
@@ -693,7 +705,6 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   if (p.cluster > 1) {
     cluster.sync();
   }
-  const int c_end = kPairs<T> ? (p.rank + 15) & ~15 : r_pad; // pairs come in sixteens of ranks
   for (int r = threadIdx.x / 8; r < TM; r += W * 4) {
     for (int c = threadIdx.x % 8; c < c_end; c += 8) {
       float sum = 0.0f;
@@ -713,12 +724,16 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
       }
       sum *= scale;
       if constexpr (kPairs<T>) {
-        const __nv_bfloat16 hi = __float2bfloat16_rn(sum);
         __nv_bfloat16 *d = reinterpret_cast<__nv_bfloat16 *>(v) +
-                           (((r / 16 * (c_end / 16) + c / 16) * 64 + r % 8 * 4 + c % 4) * 4 + (r % 16) / 8 + (c % 16) / 8 * 2) * 2 +
+                           (((r / 16 * (c_end / 16) + c / 16) * 32 * kParts + r % 8 * 4 + c % 4) * 4 + (r % 16) / 8 + (c % 16) / 8 * 2) * 2 +
                            (c % 8) / 4;
-        d[0] = hi;
-        d[256] = __float2bfloat16_rn(sum - __bfloat162float(hi));
+        float left = sum;
+#pragma unroll
+        for (int q = 0; q < kParts; q++) {
+          const __nv_bfloat16 part = __float2bfloat16_rn(left);
+          d[q * 256] = part;
+          left -= __bfloat162float(part);
+        }
       } else {
         uint32_t hi, lo;
         split(sum, hi, lo);
@@ -757,15 +772,16 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
     unsigned char *held_now = held + stage * Shape::STAGE;
     const unsigned char *src = held_now;
     stage = stage + 1 == S ? 0 : stage + 1;
-    constexpr int RS = kPairs<T> ? 16 : 8; // ranks to a product
+    constexpr int RS = kOperandRanks<T>, PARTS = kPairs<T> ? kParts : 2;
     const auto ranks = [&](int r, auto first) {
-      uint32_t hi[MT][4], lo[MT][4];
+      uint32_t parts[PARTS][MT][4];
 #pragma unroll
       for (int m = 0; m < MT; m++) {
-        const uint4 *q = operands + (m * (c_end / RS) + (r0 + r) / RS) * 64;
-        const uint4 qh = q[0], ql = q[32];
-        hi[m][0] = qh.x, hi[m][1] = qh.y, hi[m][2] = qh.z, hi[m][3] = qh.w;
-        lo[m][0] = ql.x, lo[m][1] = ql.y, lo[m][2] = ql.z, lo[m][3] = ql.w;
+#pragma unroll
+        for (int part = 0; part < PARTS; part++) {
+          const uint4 q = operands[((m * (c_end / RS) + (r0 + r) / RS) * PARTS + part) * 32];
+          parts[part][m][0] = q.x, parts[part][m][1] = q.y, parts[part][m][2] = q.z, parts[part][m][3] = q.w;
+        }
       }
       uint4 b[RS / 4];
 #pragma unroll
@@ -773,9 +789,9 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
         b[q] = r + q * 4 < RC ? shared8B(src + read_b + (r + q * 4) * 64) : make_uint4(0, 0, 0, 0);
       }
       if constexpr (kPairs<T>) {
-        mmaPairs<decltype(first)::value>(acc, hi, lo, b);
+        mmaPairs<decltype(first)::value>(acc, parts, b);
       } else {
-        mmaColumns<T, decltype(first)::value>(acc, hi, lo, b[0], b[1]);
+        mmaColumns<T, decltype(first)::value>(acc, parts[0], parts[1], b[0], b[1]);
       }
     };
     if (r0 == 0) {
@@ -840,7 +856,7 @@ void launchApply(Apply p, const LowRankRows &seg, int shift, cudaStream_t stream
   // Blocks that share a tile: as many as fit the GPU at once, eight at most. Of tiles of one row, those
   // that find others of their adapter make one; of 256 rows with 64 adapters about 80 stay.
   const long long active = MT == 1 ? std::min(slots, p.seg.adapters + slots / 16) : slots;
-  const size_t smem = ApplyShape<MT, NT>::bytes(p.rank);
+  const size_t smem = ApplyShape<MT, NT>::template bytes<T>(p.rank);
   const long long fit = std::min<long long>(ApplyShape<MT, NT>::BLOCKS, kSharedPerSm / (smem + 1024));
   p.cluster = 1;
   while (p.cluster < 8 && active * p.cluster * 2 <= fit * digitalSmCount()) {
@@ -1000,16 +1016,21 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
         for (int q = 0; q < 4; q++) {
           b[q] = shared16B(xs + (r + 4 * q) * 128);
         }
-        uint32_t hi[RT][4], lo[RT][4];
+        uint32_t parts[kParts][RT][4];
 #pragma unroll
         for (int q = 0; q < RT; q++) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float *f = uf + (r + (e >> 1) * 8) * Shape::US + q * 16 + (e & 1) * 8;
-            splitPair(f[0], f[4 * Shape::US], hi[q][e], lo[q][e]);
+            uint32_t pair[kParts];
+            splitPair(f[0], f[4 * Shape::US], pair);
+#pragma unroll
+            for (int part = 0; part < kParts; part++) {
+              parts[part][q][e] = pair[part];
+            }
           }
         }
-        mmaPairs<false>(acc, hi, lo, b);
+        mmaPairs<false>(acc, parts, b);
       }
     } else {
 #pragma unroll
