@@ -100,9 +100,7 @@ __device__ __forceinline__ RowTile findTile(const Segments &s, int slot) {
 // adapter among its 1024 neighbours, sixteen at a time, so that the adapter is read once for them; the first
 // of the sixteen keeps the tile, for the others this returns false. All warps of all blocks of a tile find the same.
 __device__ __forceinline__ bool gatherRows(const Segments &s, RowTile &tile, int lane, int list[16]) {
-  if (lane < 16) {
-    list[lane] = tile.row0 + min(lane, tile.rows - 1);
-  }
+  // every place of the list is written by one lane only: ballots order no memory
   if (tile.rows == 1 && tile.id >= 0 && tile.alone) {
     const int first = tile.seg & ~1023, end = min(first + 1024, s.n);
     int before = 0, found = 0; // of the adapter's single rows: ahead of this one, all so far
@@ -140,6 +138,8 @@ __device__ __forceinline__ bool gatherRows(const Segments &s, RowTile &tile, int
     if (lane >= tile.rows && lane < 16) {
       list[lane] = list[0];
     }
+  } else if (lane < 16) {
+    list[lane] = tile.row0 + min(lane, tile.rows - 1);
   }
   __syncwarp();
   return true;
