@@ -507,9 +507,11 @@ void launchBackward(const NormShape &sh, const NormBwd &a, const DropKey &key, i
   const size_t smem = normAhead<T>(VEC, WIDE, NS)  ? RowRing<T, NS>::bytes(normTensors(a), normThreads(sh))
                       : a.partial && !WIDE ? (size_t)sh.cols * 2 * sizeof(float)
                                            : 0;
-  if (smem > 48 * 1024) {
+  if (normAhead<T>(VEC, WIDE, NS)) {
+    // Always the most that this kernel can ask for (four tensors, 16 warps): the limit counts the kernel's static shared memory
+    // as well, and it is state of the kernel, which calls from other threads must not find lowered
     AB200_CUDA(cudaFuncSetAttribute(normBackwardKernel<T, VEC, WIDE, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (int)smem));
+                                    (int)RowRing<T, NS>::bytes(4, 512)));
   }
   AB200_CUDA(launchChained(normBackwardKernel<T, VEC, WIDE, NS>, dim3((unsigned)blocks), dim3(normThreads(sh)), smem,
                            stream, a, sh, key));
