@@ -863,9 +863,11 @@ void launchApply(Apply p, const LowRankRows &seg, int shift, cudaStream_t stream
     p.cluster *= 2;
   }
   auto kernel = lowRankApplyKernel<T, VEC, MT, NT>;
-  if (smem > 48 * 1024) {
-    AB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  }
+  // Always the most that this kernel can ask for: the limit is state of the kernel, and a call from another thread must not find
+  // it lowered between its own setting and its launch
+  constexpr int kMostRanks = NT == 8 ? kLowRankMax : 8 * NT;
+  AB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)ApplyShape<MT, NT>::template bytes<T>(kMostRanks)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(slots * p.cluster));
   cfg.blockDim = dim3(ApplyShape<MT, NT>::W * 32);
