@@ -185,20 +185,27 @@ __device__ __forceinline__ void mma16<__half>(float c[4], const uint32_t a[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// fp32 = hi + lo, hi the nearest value of 11 bits, lo the exact rest (12 bits at most, of which the
-// multiplier reads 11)
+// v, or `most` with its sign where it is larger (or NaN: the rest that it is taken from is NaN then)
+__device__ __forceinline__ float atMost(float v, float most) {
+  float r;
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+  return r;
+}
+// fp32 = hi + lo, hi the nearest finite value of 11 bits, lo the exact rest (12 bits at most, of which the
+// multiplier reads 11; 13 where hi is the largest)
 __device__ __forceinline__ void split(float v, uint32_t &hi, uint32_t &lo) {
-  hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
+  hi = __float_as_uint(atMost(__uint_as_float((__float_as_uint(v) + 0x1000u) & 0xffffe000u), __uint_as_float(0x7f7fe000u)));
   lo = __float_as_uint(v - __uint_as_float(hi));
 }
 
 // a and b as the halves of a word, in bf16, what is left of them (16 bits at most) in another, and what is left of
 // that (8 bits) in a third: fp32 = p[0] + p[1] + p[2]
 constexpr int kParts = 3;
+constexpr float kMostBf16 = 0x1.fep127f; // fp32 values above would round to infinity
 __device__ __forceinline__ void splitPair(float a, float b, uint32_t p[kParts]) {
 #pragma unroll
   for (int q = 0; q < kParts; q++) {
-    p[q] = pack2<__nv_bfloat16>(a, b);
+    p[q] = q == 0 ? pack2<__nv_bfloat16>(atMost(a, kMostBf16), atMost(b, kMostBf16)) : pack2<__nv_bfloat16>(a, b);
     const float2 f = unpack2<__nv_bfloat16>(p[q]);
     a -= f.x;
     b -= f.y;
@@ -730,7 +737,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
         float left = sum;
 #pragma unroll
         for (int q = 0; q < kParts; q++) {
-          const __nv_bfloat16 part = __float2bfloat16_rn(left);
+          const __nv_bfloat16 part = __float2bfloat16_rn(q == 0 ? atMost(left, kMostBf16) : left);
           d[q * 256] = part;
           left -= __bfloat162float(part);
         }
