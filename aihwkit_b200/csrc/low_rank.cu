@@ -170,20 +170,34 @@ __device__ __forceinline__ void loadMatrices(uint32_t src, uint32_t r[4]) {
                : "memory");
 }
 template <typename T>
-__device__ __forceinline__ void mma16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16<__nv_bfloat16>(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},"
-               "{%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
 }
-template <>
-__device__ __forceinline__ void mma16<__half>(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},"
-               "{%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+template <typename T>
+__device__ __forceinline__ void mma16First(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  }
+}
+template <bool SET> __device__ __forceinline__ void setOrAdd(float c[4], const float d[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    c[e] = SET ? d[e] : c[e] + d[e];
+  }
 }
 // v, or `most` with its sign where it is larger (or NaN: the rest that it is taken from is NaN then)
 __device__ __forceinline__ float atMost(float v, float most) {
@@ -255,15 +269,24 @@ template <typename T> __device__ __forceinline__ float elemOf(const uint4 &q, in
   }
 }
 
+// The matrix unit cuts off what an addition shifts out of its sum, up to 2^-22 of it and always toward zero: with one sum
+// going through all products of a row of 16384 positive terms that was 5e-6 of the result, in one direction (65536: 2e-5). So
+// it adds up few products at a time (a step's 32 elements of 16-bit types, half a step's eight of fp32 and their three
+// terms), and those sums are added by additions that round.
+//
 // acc[i][j] += x_i f_j for a step of 64 bytes along k, whose halves h have the operands x[i][h][0..3] and
-// f[j][2 h], f[j][2 h + 1]. Each term goes through all fragments before the next: products into one sum
+// f[j][2 h], f[j][2 h + 1]. Each term goes through some fragments before the next: products into one sum
 // wait for each other.
 template <typename T, int MT, int NT>
 __device__ __forceinline__ void mmaStep(float (&acc)[MT][NT][4], uint32_t (&x)[MT][2][4], const uint32_t (&f)[NT][4]) {
+  if constexpr (sizeof(T) == 4) {
+    // both halves in one sum where the registers hold the sums of all fragments
+    constexpr bool BOTH = MT * NT <= 8;
+    constexpr int G = BOTH ? NT : 2;
+    float sum[MT][G][4];
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    if constexpr (sizeof(T) == 4) {
-      uint32_t xl[MT][4], fh[NT][2], fl[NT][2];
+    for (int h = 0; h < 2; h++) {
+      uint32_t xl[MT][4];
 #pragma unroll
       for (int i = 0; i < MT; i++) {
 #pragma unroll
@@ -272,36 +295,71 @@ __device__ __forceinline__ void mmaStep(float (&acc)[MT][NT][4], uint32_t (&x)[M
         }
       }
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        split(__uint_as_float(f[j][2 * h]), fh[j][0], fl[j][0]);
-        split(__uint_as_float(f[j][2 * h + 1]), fh[j][1], fl[j][1]);
-      }
+      for (int j0 = 0; j0 < NT; j0 += G) {
+        uint32_t fh[G][2], fl[G][2];
 #pragma unroll
-      for (int term = 0; term < 3; term++) {
+        for (int j = 0; j < G; j++) {
+          split(__uint_as_float(f[j0 + j][2 * h]), fh[j][0], fl[j][0]);
+          split(__uint_as_float(f[j0 + j][2 * h + 1]), fh[j][1], fl[j][1]);
+        }
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
+        for (int term = 0; term < 3; term++) {
 #pragma unroll
-          for (int i = 0; i < MT; i++) {
-            mmaTf32(acc[i][j], term == 0 ? xl[i] : x[i][h], term == 1 ? fl[j][0] : fh[j][0], term == 1 ? fl[j][1] : fh[j][1]);
+          for (int j = 0; j < G; j++) {
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+              if (term == 0 && (h == 0 || !BOTH)) {
+                mmaTf32First(sum[i][j], xl[i], fh[j][0], fh[j][1]);
+              } else {
+                mmaTf32(sum[i][j], term == 0 ? xl[i] : x[i][h], term == 1 ? fl[j][0] : fh[j][0], term == 1 ? fl[j][1] : fh[j][1]);
+              }
+            }
+          }
+        }
+        if (h == 1 || !BOTH) {
+#pragma unroll
+          for (int j = 0; j < G; j++) {
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+              setOrAdd<false>(acc[i][j0 + j], sum[i][j]);
+            }
           }
         }
       }
-    } else {
+    }
+  } else {
+    constexpr int G = MT * NT <= 4 ? NT : MT >= 4 ? 1 : 4 / MT; // columns' fragments at a time
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
+    for (int j0 = 0; j0 < NT; j0 += G) {
+      float sum[MT][G][4];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+#pragma unroll
+          for (int i = 0; i < MT; i++) {
+            if (h == 0) {
+              mma16First<T>(sum[i][j], x[i][0], f[j0 + j][0], f[j0 + j][1]);
+            } else {
+              mma16<T>(sum[i][j], x[i][1], f[j0 + j][2], f[j0 + j][3]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < G; j++) {
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-          mma16<T>(acc[i][j], x[i][h], f[j][2 * h], f[j][2 * h + 1]);
+          setOrAdd<false>(acc[i][j0 + j], sum[i][j]);
         }
       }
     }
   }
 }
-// acc[i][j] += (hi_i + lo_i) b_j for the neighbouring columns j of one thread: b0 from row t of the
-// factor, b1 from row t + 4. FIRST: acc is set, not added to
-template <typename T, bool FIRST, int MT, int NJ>
-__device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], const uint32_t (&hi)[MT][4], const uint32_t (&lo)[MT][4],
-                                           const uint4 &b0, const uint4 &b1) {
+// acc[i][j] += v_i b_j for the neighbouring columns j of one thread: b0 from row t of the factor, b1 from row t + 4;
+// partsOf(i, parts) gives the upper and the lower part of v_i. FIRST: acc is set, not added to
+template <typename T, bool FIRST, int MT, int NJ, typename PartsOf>
+__device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], PartsOf partsOf, const uint4 &b0, const uint4 &b1) {
   uint32_t b[NJ][2], bl[NJ][2];
 #pragma unroll
   for (int j = 0; j < NJ; j++) {
@@ -314,19 +372,39 @@ __device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], const uint32
       b[j][1] = __float_as_uint(f1);
     }
   }
+  constexpr int GJ = NJ < 4 ? NJ : 4, GI = MT < 4 / GJ ? MT : 4 / GJ; // fragments at a time
 #pragma unroll
-  for (int term = 0; term < 3; term++) {
-    if (term == 1 && sizeof(T) != 4) {
-      continue; // 16-bit factors have no lower part
+  for (int i0 = 0; i0 < MT; i0 += GI) {
+    uint32_t parts[GI][2][4];
+#pragma unroll
+    for (int i = 0; i < GI; i++) {
+      partsOf(i0 + i, parts[i]);
     }
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
+    for (int j0 = 0; j0 < NJ; j0 += GJ) {
+      float sum[GI][GJ][4];
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
-        if (FIRST && term == 0) {
-          mmaTf32First(acc[i][j], lo[i], b[j][0], b[j][1]);
-        } else {
-          mmaTf32(acc[i][j], term == 0 ? lo[i] : hi[i], term == 1 ? bl[j][0] : b[j][0], term == 1 ? bl[j][1] : b[j][1]);
+      for (int term = 0; term < 3; term++) {
+        if (term == 1 && sizeof(T) != 4) {
+          continue; // 16-bit factors have no lower part
+        }
+#pragma unroll
+        for (int j = 0; j < GJ; j++) {
+#pragma unroll
+          for (int i = 0; i < GI; i++) {
+            if (term == 0) {
+              mmaTf32First(sum[i][j], parts[i][1], b[j0 + j][0], b[j0 + j][1]);
+            } else {
+              mmaTf32(sum[i][j], parts[i][0], term == 1 ? bl[j0 + j][0] : b[j0 + j][0], term == 1 ? bl[j0 + j][1] : b[j0 + j][1]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < GJ; j++) {
+#pragma unroll
+        for (int i = 0; i < GI; i++) {
+          setOrAdd<FIRST>(acc[i0 + i][j0 + j], sum[i][j]);
         }
       }
     }
@@ -335,9 +413,7 @@ __device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], const uint32
 
 // The same for bf16 and sixteen rows of the factor: rows t and t + 4 (b[0], b[1]) go as a pair, and rows t + 8 and
 // t + 12 (b[2], b[3]); the parts of their factors come in the same pairs
-template <bool FIRST, int MT, int NJ>
-__device__ __forceinline__ void mmaPairs(float (&acc)[MT][NJ][4], const uint32_t (&parts)[kParts][MT][4], const uint4 (&b)[4]) {
-  uint32_t p[NJ][2];
+template <int NJ> __device__ __forceinline__ void pairColumns(const uint4 (&b)[4], uint32_t (&p)[NJ][2]) {
 #pragma unroll
   for (int j = 0; j < NJ; j++) {
     const int w = j >> 1;
@@ -348,17 +424,26 @@ __device__ __forceinline__ void mmaPairs(float (&acc)[MT][NJ][4], const uint32_t
       p[j][h] = __byte_perm(w == 0 ? x.x : w == 1 ? x.y : w == 2 ? x.z : x.w, w == 0 ? y.x : w == 1 ? y.y : w == 2 ? y.z : y.w, pick);
     }
   }
+}
+template <bool FIRST, int NJ>
+__device__ __forceinline__ void mmaPairs(float (&acc)[NJ][4], const uint32_t (&parts)[kParts][4], const uint32_t (&p)[NJ][2]) {
 #pragma unroll
-  for (int part = kParts - 1; part >= 0; part--) {
+  for (int j0 = 0; j0 < NJ; j0 += 4) {
+    float sum[4][4];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
+    for (int part = kParts - 1; part >= 0; part--) {
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
-        if (FIRST && part == kParts - 1) {
-          acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
+      for (int j = 0; j < 4; j++) {
+        if (part == kParts - 1) {
+          mma16First<__nv_bfloat16>(sum[j], parts[part], p[j0 + j][0], p[j0 + j][1]);
+        } else {
+          mma16<__nv_bfloat16>(sum[j], parts[part], p[j0 + j][0], p[j0 + j][1]);
         }
-        mma16<__nv_bfloat16>(acc[i][j], parts[part][i], p[j][0], p[j][1]);
       }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      setOrAdd<FIRST>(acc[j0 + j], sum[j]);
     }
   }
 }
@@ -781,27 +866,32 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
     stage = stage + 1 == S ? 0 : stage + 1;
     constexpr int RS = kOperandRanks<T>, PARTS = kPairs<T> ? kParts : 2;
     const auto ranks = [&](int r, auto first) {
-      uint32_t parts[PARTS][MT][4];
-#pragma unroll
-      for (int m = 0; m < MT; m++) {
+      const auto partsOf = [&](int m, uint32_t (&parts)[PARTS][4]) {
 #pragma unroll
         for (int part = 0; part < PARTS; part++) {
           const uint4 q = operands[((m * (c_end / RS) + (r0 + r) / RS) * PARTS + part) * 32];
-          parts[part][m][0] = q.x, parts[part][m][1] = q.y, parts[part][m][2] = q.z, parts[part][m][3] = q.w;
+          parts[part][0] = q.x, parts[part][1] = q.y, parts[part][2] = q.z, parts[part][3] = q.w;
         }
-      }
+      };
       uint4 b[RS / 4];
 #pragma unroll
       for (int q = 0; q < RS / 4; q++) {
         b[q] = r + q * 4 < RC ? shared8B(src + read_b + (r + q * 4) * 64) : make_uint4(0, 0, 0, 0);
       }
       if constexpr (kPairs<T>) {
-        mmaPairs<decltype(first)::value>(acc, parts, b);
+        uint32_t pairs[NJ][2];
+        pairColumns(b, pairs);
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+          uint32_t parts[PARTS][4];
+          partsOf(m, parts);
+          mmaPairs<decltype(first)::value>(acc[m], parts, pairs);
+        }
       } else {
-        mmaColumns<T, decltype(first)::value>(acc, parts[0], parts[1], b[0], b[1]);
+        mmaColumns<T, decltype(first)::value>(acc, partsOf, b[0], b[1]);
       }
     };
-    if (r0 == 0) {
+    if (NT < 8 || r0 == 0) { // kernels of fewer than 64 ranks have them all in one pass
       ranks(0, std::true_type());
     } else {
       ranks(0, std::false_type());
@@ -812,7 +902,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
         ranks(r, std::false_type());
       }
     }
-    if (r0 + RC < p.rank) {
+    if (NT == 8 && r0 + RC < p.rank) {
       r0 += RC;
       continue;
     }
@@ -1018,16 +1108,18 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
     const unsigned char *xs = src + warp * Shape::XB + t * 128 + (g ^ (2 * t)) * 16;
     const float *uf = us + t * Shape::US + g;
     if constexpr (kPairs<T>) {
-#pragma unroll
+#pragma unroll 1
       for (int r = 0; r < kGradRows; r += 16) {
         uint4 b[4];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
           b[q] = shared16B(xs + (r + 4 * q) * 128);
         }
-        uint32_t parts[kParts][RT][4];
+        uint32_t pairs[NJ][2];
+        pairColumns(b, pairs);
 #pragma unroll
         for (int q = 0; q < RT; q++) {
+          uint32_t parts[kParts][4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float *f = uf + (r + (e >> 1) * 8) * Shape::US + q * 16 + (e & 1) * 8;
@@ -1035,25 +1127,23 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
             splitPair(f[0], f[4 * Shape::US], pair);
 #pragma unroll
             for (int part = 0; part < kParts; part++) {
-              parts[part][q][e] = pair[part];
+              parts[part][e] = pair[part];
             }
           }
+          mmaPairs<false>(acc[q], parts, pairs);
         }
-        mmaPairs<false>(acc, parts, b);
       }
     } else {
-#pragma unroll
+#pragma unroll 1
       for (int r = 0; r < kGradRows; r += 8) {
         const uint4 x0 = shared16B(xs + r * 128), x1 = shared16B(xs + (r + 4) * 128);
-        uint32_t hi[RT][4], lo[RT][4];
-#pragma unroll
-        for (int q = 0; q < RT; q++) {
+        const auto partsOf = [&](int q, uint32_t (&parts)[2][4]) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            split(uf[(r + (e >> 1) * 4) * Shape::US + q * 16 + (e & 1) * 8], hi[q][e], lo[q][e]);
+            split(uf[(r + (e >> 1) * 4) * Shape::US + q * 16 + (e & 1) * 8], parts[0][e], parts[1][e]);
           }
-        }
-        mmaColumns<T, false>(acc, hi, lo, x0, x1);
+        };
+        mmaColumns<T, false>(acc, partsOf, x0, x1);
       }
     }
   }
