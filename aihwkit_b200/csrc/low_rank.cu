@@ -1018,6 +1018,7 @@ struct Grad {
   int *slot_id;      // [slots]
   int width[2];
   int rank, rank_passes;
+  int block0; // first block of columns of this launch
 };
 
 constexpr int kGradWarps = 4, kGradRows = 32, kGradStages = 3;
@@ -1038,17 +1039,18 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
   waitForLaunchBefore();
   const int side = blockIdx.z / p.rank_passes, r0 = (blockIdx.z % p.rank_passes) * 16 * RT;
   const RowTile tile = findTile(p.seg, blockIdx.x);
-  if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
+  const int column_block = p.block0 + (int)blockIdx.y;
+  if (column_block == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
     p.slot_id[blockIdx.x] = tile.rows > 0 ? tile.id : -1;
   }
   const int width = side ? p.width[1] : p.width[0];
   const long long ld = side ? p.x_ld[1] : p.x_ld[0];
   float *partial = side ? p.partial[1] : p.partial[0];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  if (tile.rows <= 0 || tile.id < 0 || partial == nullptr || (int)blockIdx.y * kGradWarps * UC >= width) {
+  if (tile.rows <= 0 || tile.id < 0 || partial == nullptr || column_block * kGradWarps * UC >= width) {
     return; // all threads alike
   }
-  const int unit = blockIdx.y * kGradWarps + warp; // may lie past the width: all its columns are zeros then
+  const int unit = column_block * kGradWarps + warp; // may lie past the width: all its columns are zeros then
   const T *x = (const T *)(side ? p.x[1] : p.x[0]) + tile.row0 * ld;
   const float *u = (side ? p.u[1] : p.u[0]) + (long long)tile.row0 * p.rank + r0;
   const int ranks = min(p.rank - r0, 16 * RT);
@@ -1250,12 +1252,16 @@ template <typename T, bool VEC> void launchGrad(Grad p, long long slots, cudaStr
   const int uc = 8 * (16 / (int)sizeof(T)) * kGradWarps;
   const int rt = p.rank <= 16 ? 1 : p.rank <= 32 ? 2 : 4;
   p.rank_passes = (p.rank + 16 * rt - 1) / (16 * rt);
-  const dim3 grid((unsigned)slots, (unsigned)((widest + uc - 1) / uc), (unsigned)(2 * p.rank_passes));
   auto kernel = rt == 1 ? lowRankGradKernel<T, VEC, 1> : rt == 2 ? lowRankGradKernel<T, VEC, 2> : lowRankGradKernel<T, VEC, 4>;
   const int smem = rt == 1 ? GradShape<1>::BYTES : rt == 2 ? GradShape<2>::BYTES : GradShape<4>::BYTES;
   AB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  AB200_CUDA(launchChained(kernel, grid, dim3(kGradWarps * 32), smem, st, p));
-  AB200_LAUNCH_CHECK();
+  // a grid's second dimension takes 65535 blocks: rows of more than 8388480 fp32 columns go in parts
+  const int blocks = (widest + uc - 1) / uc;
+  for (p.block0 = 0; p.block0 < blocks; p.block0 += 65535) {
+    const dim3 grid((unsigned)slots, (unsigned)std::min(blocks - p.block0, 65535), (unsigned)(2 * p.rank_passes));
+    AB200_CUDA(launchChained(kernel, grid, dim3(kGradWarps * 32), smem, st, p));
+    AB200_LAUNCH_CHECK();
+  }
 }
 template <typename T>
 void gradOfType(const Grad &p, const LowRankGradArgs &a, long long slots, bool vec, cudaStream_t st) {
