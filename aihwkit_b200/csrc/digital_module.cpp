@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 
+#include <algorithm>
 #include <sstream>
 #include <stdexcept>
 
@@ -146,24 +147,25 @@ struct Wanted {
   size_t next;
   bool operator()(const Tensor &input) { return input.defined() && ctx->needs_input_grad(next++); }
 };
-// Gradients of a backward pass that is itself recorded: differentiating them by anything that they were made
-// from raises.
-variable_list once(variable_list grads, const variable_list &made_from) {
-  if (!at::GradMode::is_enabled()) {
-    return grads;
+// A gradient of a backward pass that is itself recorded: differentiating it raises by anything that it was made from, the
+// incoming gradients and those inputs of the forward call whose places among the node's inputs are given (-1: missing). The
+// node knows its inputs by their edges, whether or not it has kept their values.
+Tensor once(Tensor g, const variable_list &incoming, std::initializer_list<int> places) {
+  if (!g.defined() || !at::GradMode::is_enabled()) {
+    return g;
   }
-  auto node = std::make_shared<torch::autograd::Error>("the digital operators' gradients are not differentiable again",
-                                                       torch::autograd::collect_next_edges(made_from));
-  for (Tensor &g : grads) {
-    if (g.defined() && !g.requires_grad()) { // one that is passed on has its own history, one that appears twice has it by now
-      torch::autograd::set_history(g, node);
+  torch::autograd::edge_list edges = torch::autograd::collect_next_edges(incoming);
+  const auto node = torch::autograd::get_current_node();
+  for (int place : places) {
+    if (place >= 0) {
+      edges.push_back(node->next_edge(place));
     }
   }
-  return grads;
-}
-variable_list joined(variable_list a, const variable_list &b) {
-  a.insert(a.end(), b.begin(), b.end());
-  return a;
+  if (std::any_of(edges.begin(), edges.end(), [](const torch::autograd::Edge &e) { return e.is_valid(); })) {
+    torch::autograd::set_history(g, std::make_shared<torch::autograd::Error>(
+                                        "the digital operators' gradients are not differentiable again", std::move(edges)));
+  }
+  return g;
 }
 
 // ---- dropout ----------------------------------------------------------------------------------
@@ -192,7 +194,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
                       (uint32_t)ctx->saved_data["call"].toInt()};
     Tensor dx;
     if (ctx->needs_input_grad(0)) {
-      dx = once({dropoutCompute(gs[0], r, Tensor())}, gs)[0];
+      dx = once(dropoutCompute(gs[0], r, Tensor()), gs, {});
     }
     const bool need_res = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1);
     return {dx, need_res ? gs[0] : Tensor(), Tensor(), Tensor(), Tensor()};
@@ -309,7 +311,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const bool need_w = wanted(s[1]), need_b = wanted(s[2]);
     const NormGrads g = normGradCompute(gs[0], Tensor(), s[0], Tensor(), s[1], s[2], s[3], {0.0, 0, 0},
                                         ctx->needs_input_grad(0), false, need_w, need_b);
-    return once({g.dh, g.dw, g.db, Tensor()}, joined(gs, {s[0], s[1]}));
+    return {once(g.dh, gs, {0, s[1].defined() ? 1 : -1}), once(g.dw, gs, {0}), once(g.db, gs, {}), Tensor()};
   }
 };
 // h = residual + dropout(x), y = norm(h). The backward pass needs h as it went into the norm: an fp32 h is
@@ -340,14 +342,15 @@ struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
     if (gs[0].defined()) {
       g = normGradCompute(gs[0], gs[1], s[0], s[1], s[2], s[3], s[4], r, need_res || (need_x && !dropped),
                           need_x && dropped, need_w, need_b);
+      const int w = s[2].defined() ? 2 : -1;
+      g = {once(g.dh, gs, {0, 1, w}), once(g.dx, gs, {0, 1, w}), once(g.dw, {gs[0]}, {0, 1}), once(g.db, {gs[0]}, {})};
     } else if (gs[1].defined()) {
-      g.dh = gs[1];
+      g.dh = gs[1]; // the caller's own tensor, with whatever history it has
       if (need_x && dropped) {
-        g.dx = dropoutCompute(gs[1], r, Tensor());
+        g.dx = once(dropoutCompute(gs[1], r, Tensor()), gs, {});
       }
     }
-    variable_list out = once({need_x ? (dropped ? g.dx : g.dh) : Tensor(), need_res ? g.dh : Tensor(), g.dw, g.db},
-                             joined(gs, {s[0], s[1], s[2]}));
+    variable_list out = {need_x ? (dropped ? g.dx : g.dh) : Tensor(), need_res ? g.dh : Tensor(), g.dw, g.db};
     out.resize(8);
     return out;
   }
@@ -430,8 +433,9 @@ struct LowRankAdd : torch::autograd::Function<LowRankAdd> {
                                 (int)n, ids.data_ptr<int>(), (const int32_t *)ptr(starts), (int)ids.numel(), rows,
                                 (int)rank, (int)a.size(0), typeCode(gy, "gy"), ptr(work), stream()));
     }
-    const variable_list g = once({dx, da, db}, joined(gs, {x, a, b}));
-    return {ctx->needs_input_grad(0) ? gy : Tensor(), g[0], g[1], g[2], Tensor(), Tensor(), Tensor()};
+    // of the inputs base, x, a, b
+    return {ctx->needs_input_grad(0) ? gy : Tensor(), once(dx, gs, {2, 3}), once(da, gs, {1, 3}), once(db, gs, {1, 2}), Tensor(),
+            Tensor(), Tensor()};
   }
 };
 // Whether two tensors may share memory: their address ranges meet, and they are not columns of one
