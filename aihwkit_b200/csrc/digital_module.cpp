@@ -8,6 +8,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <algorithm>
 #include <sstream>
@@ -45,6 +49,19 @@ int typeCode(const Tensor &t, const char *name) {
     REFUSE(true, name << " must be a float32, float16 or bfloat16 tensor, got " << t.scalar_type());
   }
   return 0;
+}
+// The kernels write results through plain pointers, which forward-mode differentiation and tracers do not see: a result would have
+// no tangent (a derivative of zero), a trace the result's allocation and nothing that fills it.
+void checkModes(std::initializer_list<const Tensor *> tensors) {
+  REFUSE(torch::jit::tracer::isTracing() ||
+             c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+         "the digital operators cannot be traced");
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+    return;
+  }
+  for (const Tensor *t : tensors) {
+    REFUSE(torch::autograd::isFwGradDefined(*t), "the digital operators have no forward-mode derivative: detach the dual tensor");
+  }
 }
 void checkCuda(const Tensor &t, const char *name) {
   typeCode(t, name);
@@ -202,9 +219,10 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 Tensor dropout(const Tensor &x, double p, const py::int_ &seed, const py::int_ &call,
                const std::optional<Tensor> &residual_) {
+  const Tensor residual = optional(residual_);
+  checkModes({&x, &residual});
   checkCuda(x, "x");
   checkRowsOf(x);
-  const Tensor residual = optional(residual_);
   if (residual.defined()) {
     checkSame(residual, "residual", x);
   }
@@ -217,6 +235,7 @@ Tensor dropout(const Tensor &x, double p, const py::int_ &seed, const py::int_ &
 
 // ---- layer norm -------------------------------------------------------------------------------
 void checkNorm(const Tensor &x, const Tensor &residual, const Tensor &weight, const Tensor &bias) {
+  checkModes({&x, &residual, &weight, &bias});
   checkCuda(x, "x");
   checkRowsOf(x);
   if (residual.defined()) {
@@ -467,6 +486,7 @@ bool overlap(const Tensor &s, const Tensor &t) {
 Tensor lowRankAdd(const Tensor &base, const Tensor &x, const Tensor &a, const Tensor &b, const Tensor &scale,
                   const Tensor &ids, const std::optional<Tensor> &starts_, const std::optional<Tensor> &out_) {
   const Tensor starts = optional(starts_), out = optional(out_);
+  checkModes({&base, &x, &a, &b, &scale, &out});
   checkCuda(x, "x");
   checkLike(base, "base", x);
   checkLike(a, "a", x);
