@@ -26,7 +26,8 @@ Two ways to use N ranks (``--shard``):
 With ``--adapters N`` every analog layer has a pool of N low-rank adapters beside its tiles, the sequences of the
 batch use them in turn, and the digital parts of the blocks (residual sums, LayerNorm, dropout in training) run on the
 library's own kernels (:mod:`aihwkit_b200.digital`).  ``--adapt-steps K`` then takes K training steps on the adapters and
-the norms: the conductances stay as they were programmed, gradients pass the tiles through their transposed product.
+the norms, in one process: the conductances stay as they were programmed, gradients pass the tiles through their transposed
+product.
 
 Prints one JSON line (rank 0): tokens/s of the whole forward, the share of the analog layers, and
 their logical TFLOP/s.
@@ -269,7 +270,12 @@ class AnalogGPT2:
 
 def adapt(model: AnalogGPT2, ids: torch.Tensor, n_adapters: int, steps: int, lr: float = 1e-3, p: float = 0.1) -> dict:
     """Training steps on the adapters and norms, one sequence at a time (the logits of one are 0.2 GB at 1024 tokens),
-    gradients of the batch added up; returns the time of a step and the losses."""
+    gradients of the batch added up; returns the time of a step and the losses.  One process only: nothing here adds the
+    gradients of several ranks up, and each would go on with a model of its own."""
+    import torch.distributed as dist
+
+    if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
+        raise RuntimeError("adaptation runs in one process: gradients are not added up over ranks")
     weights = model.trained()
     for t in weights:
         t.requires_grad_()
@@ -305,10 +311,13 @@ def main(argv=None):
                     help="N > 1: split the sequences over the ranks, or the tiles of every analog layer")
     ap.add_argument("--adapters", type=int, default=0, help="low-rank adapters beside every analog layer")
     ap.add_argument("--rank", type=int, default=16, help="rank of the adapters")
-    ap.add_argument("--adapt-steps", type=int, default=0, help="training steps on adapters and norms after the forward passes")
+    ap.add_argument("--adapt-steps", type=int, default=0, help="training steps on adapters and norms after the forward passes (one process)")
     args = ap.parse_args(argv)
+    world = int(os.environ.get("WORLD_SIZE", "1"))
     if args.adapt_steps and not args.adapters:
         raise SystemExit("--adapt-steps needs --adapters")
+    if args.adapt_steps and world > 1:
+        raise SystemExit("--adapt-steps runs in one process: gradients are not added up over ranks")
 
     import torch.distributed as dist
 
@@ -316,7 +325,6 @@ def main(argv=None):
 
     if not torch.cuda.is_available():
         raise RuntimeError("needs a CUDA device: the analog tiles have no CPU path")
-    world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
     local_rank = int(os.environ.get("LOCAL_RANK", "0"))
     torch.cuda.set_device(local_rank)

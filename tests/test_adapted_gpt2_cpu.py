@@ -1,0 +1,18 @@
+"""Options of the GPT-2-shaped command with adapters that are refused before a device is looked for."""
+
+import pytest
+
+from aihwkit_b200 import gpt2_inference as G
+
+
+def test_adaptation_of_several_ranks_is_refused(monkeypatch):
+    """Each rank would train a model of its own."""
+    import torch.distributed as dist
+
+    monkeypatch.setenv("WORLD_SIZE", "2")
+    with pytest.raises(SystemExit, match="one process"):
+        G.main(["--adapters", "2", "--adapt-steps", "1"])
+    monkeypatch.setattr(dist, "is_initialized", lambda: True)
+    monkeypatch.setattr(dist, "get_world_size", lambda group=None: 2)
+    with pytest.raises(RuntimeError, match="one process"):
+        G.adapt(None, None, 2, 1)
