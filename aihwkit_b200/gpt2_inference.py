@@ -268,6 +268,12 @@ class AnalogGPT2:
         return sum(lin.n_tiles for blk in self.blocks for lin in blk.linears())
 
 
+def sequence_adapters(first: int, count: int, n_adapters: int, device) -> torch.Tensor:
+    """Adapters of the batch's sequences ``first``, ``first + 1``, ... (``count`` of them): in turn over the whole batch, however
+    many ranks share it."""
+    return torch.arange(first, first + count, device=device) % n_adapters
+
+
 def adapt(model: AnalogGPT2, ids: torch.Tensor, n_adapters: int, steps: int, lr: float = 1e-3, p: float = 0.1) -> dict:
     """Training steps on the adapters and norms, one sequence at a time (the logits of one are 0.2 GB at 1024 tokens),
     gradients of the batch added up; returns the time of a step and the losses.  One process only: nothing here adds the
@@ -347,7 +353,7 @@ def main(argv=None):
     ids = ids_host.to(model.device)
     run = None
     if args.adapters:
-        run = Adaptation(torch.arange(local_batch, device=model.device) % args.adapters, args.seq)
+        run = Adaptation(sequence_adapters(rank * local_batch, local_batch, args.adapters, model.device), args.seq)
 
     def barrier():
         if world > 1:

@@ -16,3 +16,11 @@ def test_adaptation_of_several_ranks_is_refused(monkeypatch):
     monkeypatch.setattr(dist, "get_world_size", lambda group=None: 2)
     with pytest.raises(RuntimeError, match="one process"):
         G.adapt(None, None, 2, 1)
+
+
+@pytest.mark.parametrize("world", [1, 2, 4, 8])
+@pytest.mark.parametrize("adapters", [1, 3, 4, 16])
+def test_sequences_use_the_adapters_in_turn_over_all_ranks(world, adapters):
+    local = 16 // world
+    got = [int(i) for rank in range(world) for i in G.sequence_adapters(rank * local, local, adapters, "cpu")]
+    assert got == [j % adapters for j in range(16)]
