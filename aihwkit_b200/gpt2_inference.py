@@ -282,6 +282,8 @@ def adapt(model: AnalogGPT2, ids: torch.Tensor, n_adapters: int, steps: int, lr:
 
     if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
         raise RuntimeError("adaptation runs in one process: gradients are not added up over ranks")
+    if ids.size(1) < 2:
+        raise RuntimeError("adaptation needs sequences of at least two tokens: the next one is what is learned")
     weights = model.trained()
     for t in weights:
         t.requires_grad_()
@@ -324,6 +326,8 @@ def main(argv=None):
         raise SystemExit("--adapt-steps needs --adapters")
     if args.adapt_steps and world > 1:
         raise SystemExit("--adapt-steps runs in one process: gradients are not added up over ranks")
+    if args.adapt_steps and args.seq < 2:
+        raise SystemExit("--adapt-steps needs sequences of at least two tokens")
 
     import torch.distributed as dist
 

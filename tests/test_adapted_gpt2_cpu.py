@@ -24,3 +24,13 @@ def test_sequences_use_the_adapters_in_turn_over_all_ranks(world, adapters):
     local = 16 // world
     got = [int(i) for rank in range(world) for i in G.sequence_adapters(rank * local, local, adapters, "cpu")]
     assert got == [j % adapters for j in range(16)]
+
+
+def test_adaptation_without_a_next_token_is_refused():
+    """The mean over no tokens is not a number, and a step on it would leave none of the weights one."""
+    import torch
+
+    with pytest.raises(SystemExit, match="two tokens"):
+        G.main(["--adapters", "2", "--adapt-steps", "1", "--seq", "1"])
+    with pytest.raises(RuntimeError, match="two tokens"):
+        G.adapt(None, torch.zeros(2, 1, dtype=torch.long), 2, 1)
