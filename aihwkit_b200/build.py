@@ -3,7 +3,8 @@
     python -m aihwkit_b200.build [--force] [--verbose]
 
 nvcc cross-compiles without a GPU.  The library links cudart statically and has no torch
-dependency; ``libcuda`` entry points (tensor maps) are resolved at run time.
+dependency; ``libcuda`` entry points (tensor maps) are resolved at run time.  Where torch is installed, the command also
+builds ``ab200_digital.so``, the torch binding of the digital operators (``build_digital``).
 """
 
 from __future__ import annotations
@@ -76,7 +77,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
-    _build_digital(force)
     if verbose:
         for src, log in logs.items():
             print(f"== {os.path.basename(src)}\n{log}")
@@ -86,17 +86,16 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return OUT
 
 
-def _build_digital(force: bool) -> None:
-    """Compile ``csrc/digital_module.cpp``, the torch binding of ``aihwkit_b200.digital`` over the C ABI."""
-    src = os.path.join(CSRC, "digital_module.cpp")
-    include = os.path.join(os.path.dirname(HERE), "include")
-    if not force and not _stale(DIGITAL_OUT, [src, os.path.join(include, "aihwkit_b200.h")]):
-        return
+def build_digital(force: bool = False) -> str:
+    """Compile ``csrc/digital_module.cpp``, the torch binding of ``aihwkit_b200.digital`` over the C ABI; the library has to be
+    there.  It is built again when its sources, the compiler's command line or the version of torch or Python change."""
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
+    src = os.path.join(CSRC, "digital_module.cpp")
+    include = os.path.join(os.path.dirname(HERE), "include")
     cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.isabs(_nvcc()) else "/usr/local/cuda"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=ab200_digital",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", DIGITAL_OUT, f"-I{include}",
@@ -104,9 +103,21 @@ def _build_digital(force: bool) -> None:
     cmd += [f"-I{d}" for d in include_paths()] + [f"-L{d}" for d in library_paths()]
     cmd += [f"-L{CSRC}", "-laihwkit_b200", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
             "-ltorch_cuda", "-ltorch_python"]
+    made_by = "\n".join([torch.__version__, sys.version] + cmd)
+    record = os.path.join(OBJ, "ab200_digital.txt")
+    known = ""
+    if os.path.exists(record):
+        with open(record, encoding="utf-8") as f:
+            known = f.read()
+    if not force and known == made_by and not _stale(DIGITAL_OUT, [src, os.path.join(include, "aihwkit_b200.h")]):
+        return DIGITAL_OUT
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for {src}:\n{res.stdout}\n{res.stderr}")
+    os.makedirs(OBJ, exist_ok=True)
+    with open(record, "w", encoding="utf-8") as f:
+        f.write(made_by)
+    return DIGITAL_OUT
 
 
 def build_pybind(verbose: bool = False):
@@ -138,4 +149,8 @@ if __name__ == "__main__":
     ap.add_argument("--verbose", action="store_true")
     a = ap.parse_args()
     print(build(a.force, a.verbose))
+    try:
+        print(build_digital(a.force))
+    except ModuleNotFoundError as exc:
+        print(f"without the binding of the digital operators: {exc}")
     sys.exit(0)
