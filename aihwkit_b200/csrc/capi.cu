@@ -1080,6 +1080,15 @@ void digitalPointer(const char *what, const char *name, const void *p, long long
     AB200_FATAL(what << ": " << name << " is null");
   }
 }
+// addresses that are no multiple of what a kernel reads or writes at once would fault on the device
+void digitalAligned(const char *what, size_t bytes, std::initializer_list<std::pair<const char *, const void *>> pointers) {
+  for (const auto &q : pointers) {
+    if ((uintptr_t)q.second % bytes != 0) {
+      AB200_FATAL(what << ": " << q.first << " must lie on a multiple of " << bytes << " bytes");
+    }
+  }
+}
+size_t digitalSize(int dtype) { return dtype == AB200_DTYPE_F32 ? 4 : 2; }
 // distances between rows: not negative, and of outputs at least a row
 void digitalStrides(const char *what, long long rows, std::initializer_list<long long> inputs,
                     std::initializer_list<std::pair<long long, int>> outputs) {
@@ -1122,6 +1131,7 @@ int ab200_dropout(const void *x, long long x_stride, const void *residual, long 
   digitalRows("dropout", rows, cols, 1 << 30);
   digitalPointer("dropout", "x", x, rows);
   digitalPointer("dropout", "y", y, rows);
+  digitalAligned("dropout", digitalSize(dtype), {{"x", x}, {"residual", residual}, {"y", y}});
   digitalStrides("dropout", rows, {x_stride, residual_stride}, {{y_stride, cols}});
   ab200::dropoutApply({x, x_stride}, {residual, residual_stride}, {y, y_stride}, rows, cols, dtype,
                       digitalDrop("dropout", p, seed, call), (cudaStream_t)stream);
@@ -1141,6 +1151,9 @@ int ab200_layer_norm_forward(const void *x, long long x_stride, const void *resi
   if ((mean == nullptr) != (rstd == nullptr)) {
     AB200_FATAL("layer_norm: mean and rstd are wanted together or not at all");
   }
+  digitalAligned("layer_norm", digitalSize(dtype), {{"x", x}, {"residual", residual}, {"y", y}, {"h", h}});
+  digitalAligned("layer_norm", digitalSize(param_dtype), {{"weight", weight}, {"bias", bias}});
+  digitalAligned("layer_norm", sizeof(float), {{"mean", mean}, {"rstd", rstd}});
   digitalStrides("layer_norm", rows, {x_stride, residual_stride}, {{y_stride, cols}, {h ? h_stride : cols, cols}});
   ab200::NormArgs a = {{x, x_stride}, {residual, residual_stride}, {y, y_stride}, {h, h_stride}, weight, bias, mean,
                        rstd, rows, cols, dtype, param_dtype, eps, digitalDrop("layer_norm", p, seed, call)};
@@ -1169,6 +1182,10 @@ int ab200_layer_norm_backward(const void *gy, long long gy_stride, const void *g
   digitalPointer("layer_norm", "x", x, rows);
   digitalPointer("layer_norm", "mean", mean, rows);
   digitalPointer("layer_norm", "rstd", rstd, rows);
+  digitalAligned("layer_norm", digitalSize(dtype),
+                 {{"gy", gy}, {"gh", gh}, {"x", x}, {"residual", residual}, {"dh", dh}, {"dx", dx}});
+  digitalAligned("layer_norm", digitalSize(param_dtype), {{"weight", weight}, {"dweight", dweight}, {"dbias", dbias}});
+  digitalAligned("layer_norm", sizeof(float), {{"mean", mean}, {"rstd", rstd}, {"workspace", workspace}});
   digitalStrides("layer_norm", rows, {gy_stride, gh_stride, x_stride, residual_stride},
                  {{dh ? dh_stride : cols, cols}, {dx ? dx_stride : cols, cols}});
   const bool params = dweight != nullptr || dbias != nullptr;
@@ -1199,6 +1216,8 @@ int ab200_low_rank_apply(const void *x, long long x_stride, const void *base, lo
   if (y != nullptr) {
     digitalPointer("low_rank", "b", b, rows);
   }
+  digitalAligned("low_rank", digitalSize(dtype), {{"x", x}, {"base", base}, {"y", y}, {"a", a}, {"b", b}});
+  digitalAligned("low_rank", 4, {{"scale", scale}, {"adapter_ids", adapter_ids}, {"row_starts", row_starts}, {"v", v}});
   digitalStrides("low_rank", rows, {x_stride, base_stride}, {{y ? y_stride : n, n}});
   if (y != nullptr && y == base && y_stride != base_stride) {
     AB200_FATAL("low_rank: y in the place of base needs base's row stride");
@@ -1237,8 +1256,11 @@ int ab200_low_rank_grad(const void *x, long long x_stride, const float *u, void 
     digitalPointer("low_rank_grad", "gy", gy, rows);
     digitalPointer("low_rank_grad", "v", v, rows);
   }
+  digitalAligned("low_rank_grad", digitalSize(dtype), {{"x", x}, {"gy", gy}, {"da", da}, {"db", db}});
+  digitalAligned("low_rank_grad", 4, {{"u", u}, {"v", v}, {"adapter_ids", adapter_ids}, {"row_starts", row_starts}});
   digitalStrides("low_rank_grad", rows, {x_stride, gy_stride}, {});
   digitalPointer("low_rank_grad", "workspace", workspace, rows);
+  digitalAligned("low_rank_grad", 16, {{"workspace", workspace}}); // partial sums are stored 16 bytes at a time
   ab200::LowRankGradArgs args = {{row_starts, adapter_ids, n_requests, rows}, {{x, x_stride}, {gy, gy_stride}}, {u, v},
                                  {da, db}, {k, n}, workspace, rank, n_adapters, dtype};
   ab200::lowRankGrad(args, (cudaStream_t)stream);

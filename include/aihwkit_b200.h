@@ -795,7 +795,8 @@ int ab200_mvm_forward_noalloc(const ab200_io_params *forward_io, const float *w_
  * (a stride of 0 repeats one row and is for inputs only). Infinities and NaN make the results not finite that
  * are summed from them, and no others. Nothing is allocated and nothing is waited
  * for; the calls can be captured into a graph. Sums, means and saved values are fp32 whatever the type,
- * results are rounded once. Outputs must not overlap inputs unless a call says so. */
+ * results are rounded once. Outputs must not overlap inputs unless a call says so. Pointers lie on multiples of
+ * their elements' size, the workspace of ab200_low_rank_grad on one of 16 bytes. */
 enum ab200_dtype { AB200_DTYPE_F32 = 0, AB200_DTYPE_F16 = 1, AB200_DTYPE_BF16 = 2 };
 
 /* y = keep ? x / (1 - p) : 0, plus `residual` where it is not null. A dropped element is 0 whatever it
