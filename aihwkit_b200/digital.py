@@ -99,6 +99,14 @@ class LowRankAdapters(torch.nn.Module):
         self.b = torch.nn.Parameter(torch.zeros(n_adapters, rank, out_features, device=device, dtype=dtype))
         self.register_buffer("scale", torch.full((n_adapters,), float(scale), device=device, dtype=torch.float32))
 
+    def _apply(self, fn, recurse=True):
+        """Conversions of the pool to another type leave ``scale`` in float32, as the calls take it."""
+        scale = self.scale
+        super()._apply(fn, recurse)
+        if self.scale.dtype != torch.float32:
+            self.scale = self.scale.float() if scale.is_meta else scale.to(self.scale.device)
+        return self
+
     @torch.no_grad()
     def set_adapter(self, index: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """Adapter ``index`` becomes ``scale * b @ a`` with ``a [r, in_features]`` and ``b [out_features, r]``, ``r`` at most
