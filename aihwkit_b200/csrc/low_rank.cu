@@ -226,12 +226,10 @@ __device__ __forceinline__ void splitPair(float a, float b, uint32_t p[kParts]) 
   }
 }
 template <typename T> constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
-// bytes of an element of v as an operand of the second product, and the ranks that a product takes
+// bytes of an element of v as an operand of the second product, and the ranks that a product takes (of the gradients: u, rows)
 template <typename T> constexpr int kOperandBytes = kPairs<T> ? 2 * kParts : 8;
 template <typename T> constexpr int kOperandRanks = kPairs<T> ? 16 : 8;
-template <typename T> __host__ __device__ __forceinline__ int operandRanks(int rank) {
-  return (rank + kOperandRanks<T> - 1) / kOperandRanks<T> * kOperandRanks<T>;
-}
+__host__ __device__ __forceinline__ int operandRanks(int rank) { return (rank + 15) & ~15; }
 
 // 16 bytes of a row: eight 16-bit or four fp32 neighbours; elements past the end read as zero
 template <typename T, bool VEC>
@@ -271,8 +269,8 @@ template <typename T> __device__ __forceinline__ float elemOf(const uint4 &q, in
 
 // The matrix unit cuts off what an addition shifts out of its sum, up to 2^-22 of it and always toward zero: with one sum
 // going through all products of a row of 16384 positive terms that was 5e-6 of the result, in one direction (65536: 2e-5). So
-// it adds up few products at a time (a step's 32 elements of 16-bit types, half a step's eight of fp32 and their three
-// terms), and those sums are added by additions that round.
+// it adds up few products at a time (a step's 32 elements of 16-bit types, its 16 of fp32 in three terms; 16 ranks, or 16 to
+// 32 rows of the gradients, the smaller parts first), and those sums are added by additions that round.
 //
 // acc[i][j] += x_i f_j for a step of 64 bytes along k, whose halves h have the operands x[i][h][0..3] and
 // f[j][2 h], f[j][2 h + 1]. Each term goes through some fragments before the next: products into one sum
@@ -356,29 +354,37 @@ __device__ __forceinline__ void mmaStep(float (&acc)[MT][NT][4], uint32_t (&x)[M
     }
   }
 }
-// acc[i][j] += v_i b_j for the neighbouring columns j of one thread: b0 from row t of the factor, b1 from row t + 4;
-// partsOf(i, parts) gives the upper and the lower part of v_i. FIRST: acc is set, not added to
-template <typename T, bool FIRST, int MT, int NJ, typename PartsOf>
-__device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], PartsOf partsOf, const uint4 &b0, const uint4 &b1) {
-  uint32_t b[NJ][2], bl[NJ][2];
+// acc[i][j] += sum over STEPS of v_i b_j for the neighbouring columns j of one thread: b0 from row t of a step's eight rows
+// of the factor, b1 from row t + 4; partsOf(step, i, parts) gives the upper and the lower part of v_i. FIRST: acc is set, not
+// added to
+template <typename T, bool FIRST, int STEPS, int MT, int NJ, typename PartsOf>
+__device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], PartsOf partsOf, const uint4 (&b0)[STEPS],
+                                           const uint4 (&b1)[STEPS]) {
+  uint32_t b[STEPS][NJ][2], bl[STEPS][NJ][2];
 #pragma unroll
-  for (int j = 0; j < NJ; j++) {
-    const float f0 = elemOf<T>(b0, j), f1 = elemOf<T>(b1, j);
-    if constexpr (sizeof(T) == 4) {
-      split(f0, b[j][0], bl[j][0]);
-      split(f1, b[j][1], bl[j][1]);
-    } else {
-      b[j][0] = __float_as_uint(f0);
-      b[j][1] = __float_as_uint(f1);
+  for (int step = 0; step < STEPS; step++) {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const float f0 = elemOf<T>(b0[step], j), f1 = elemOf<T>(b1[step], j);
+      if constexpr (sizeof(T) == 4) {
+        split(f0, b[step][j][0], bl[step][j][0]);
+        split(f1, b[step][j][1], bl[step][j][1]);
+      } else {
+        b[step][j][0] = __float_as_uint(f0);
+        b[step][j][1] = __float_as_uint(f1);
+      }
     }
   }
   constexpr int GJ = NJ < 4 ? NJ : 4, GI = MT < 4 / GJ ? MT : 4 / GJ; // fragments at a time
 #pragma unroll
   for (int i0 = 0; i0 < MT; i0 += GI) {
-    uint32_t parts[GI][2][4];
+    uint32_t parts[STEPS][GI][2][4];
 #pragma unroll
-    for (int i = 0; i < GI; i++) {
-      partsOf(i0 + i, parts[i]);
+    for (int step = 0; step < STEPS; step++) {
+#pragma unroll
+      for (int i = 0; i < GI; i++) {
+        partsOf(step, i0 + i, parts[step][i]);
+      }
     }
 #pragma unroll
     for (int j0 = 0; j0 < NJ; j0 += GJ) {
@@ -389,13 +395,18 @@ __device__ __forceinline__ void mmaColumns(float (&acc)[MT][NJ][4], PartsOf part
           continue; // 16-bit factors have no lower part
         }
 #pragma unroll
-        for (int j = 0; j < GJ; j++) {
+        for (int step = 0; step < STEPS; step++) {
 #pragma unroll
-          for (int i = 0; i < GI; i++) {
-            if (term == 0) {
-              mmaTf32First(sum[i][j], parts[i][1], b[j0 + j][0], b[j0 + j][1]);
-            } else {
-              mmaTf32(sum[i][j], parts[i][0], term == 1 ? bl[j0 + j][0] : b[j0 + j][0], term == 1 ? bl[j0 + j][1] : b[j0 + j][1]);
+          for (int j = 0; j < GJ; j++) {
+#pragma unroll
+            for (int i = 0; i < GI; i++) {
+              const uint32_t (&left)[4] = parts[step][i][term == 0 ? 1 : 0];
+              const uint32_t (&right)[2] = term == 1 ? bl[step][j0 + j] : b[step][j0 + j];
+              if (term == 0 && step == 0) {
+                mmaTf32First(sum[i][j], left, right[0], right[1]);
+              } else {
+                mmaTf32(sum[i][j], left, right[0], right[1]);
+              }
             }
           }
         }
@@ -425,19 +436,23 @@ template <int NJ> __device__ __forceinline__ void pairColumns(const uint4 (&b)[4
     }
   }
 }
-template <bool FIRST, int NJ>
-__device__ __forceinline__ void mmaPairs(float (&acc)[NJ][4], const uint32_t (&parts)[kParts][4], const uint32_t (&p)[NJ][2]) {
+template <bool FIRST, int STEPS, int NJ>
+__device__ __forceinline__ void mmaPairs(float (&acc)[NJ][4], const uint32_t (&parts)[STEPS][kParts][4],
+                                         const uint32_t (&p)[STEPS][NJ][2]) {
 #pragma unroll
   for (int j0 = 0; j0 < NJ; j0 += 4) {
     float sum[4][4];
 #pragma unroll
     for (int part = kParts - 1; part >= 0; part--) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (part == kParts - 1) {
-          mma16First<__nv_bfloat16>(sum[j], parts[part], p[j0 + j][0], p[j0 + j][1]);
-        } else {
-          mma16<__nv_bfloat16>(sum[j], parts[part], p[j0 + j][0], p[j0 + j][1]);
+      for (int step = 0; step < STEPS; step++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (part == kParts - 1 && step == 0) {
+            mma16First<__nv_bfloat16>(sum[j], parts[step][part], p[step][j0 + j][0], p[step][j0 + j][1]);
+          } else {
+            mma16<__nv_bfloat16>(sum[j], parts[step][part], p[step][j0 + j][0], p[step][j0 + j][1]);
+          }
         }
       }
     }
@@ -557,7 +572,7 @@ template <int MT, int NT> struct ApplyShape {
   static constexpr int BLOCKS = MT == 1 ? 2 : 4;
   template <typename T> static size_t bytes(int rank) {
     const int vs = ((rank + 7) & ~7) + 4;
-    return RING + SHARES + (size_t)TM * (operandRanks<T>(rank) * kOperandBytes<T> + vs * 4);
+    return RING + SHARES + (size_t)TM * (operandRanks(rank) * kOperandBytes<T> + vs * 4);
   }
 };
 
@@ -624,7 +639,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
   const int r_pad = (p.rank + 7) & ~7, vs = r_pad + 4;
   unsigned char *held = smem + warp * S * Shape::STAGE; // this warp's ring
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(held);
-  const int c_end = operandRanks<T>(p.rank);
+  const int c_end = operandRanks(p.rank);
   // v of the tile as the second product's operands: [fragment][8 ranks (bf16: 16)][parts][lane][4]
   float *v = reinterpret_cast<float *>(smem + Shape::RING);
   float *mine = v + TM * c_end * kOperandBytes<T> / 4; // [TM][vs]: this block's share of v
@@ -829,7 +844,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
       } else {
         uint32_t hi, lo;
         split(sum, hi, lo);
-        float *d = v + ((r / 16 * (r_pad / 8) + c / 8) * 64 + r % 8 * 4 + c % 4) * 4 + (r % 16) / 8 + (c % 8) / 4 * 2;
+        float *d = v + ((r / 16 * (c_end / 8) + c / 8) * 64 + r % 8 * 4 + c % 4) * 4 + (r % 16) / 8 + (c % 8) / 4 * 2;
         d[0] = __uint_as_float(hi);
         d[128] = __uint_as_float(lo);
       }
@@ -865,30 +880,37 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
     const unsigned char *src = held_now;
     stage = stage + 1 == S ? 0 : stage + 1;
     constexpr int RS = kOperandRanks<T>, PARTS = kPairs<T> ? kParts : 2;
+    constexpr int STEPS = kPairs<T> || NT == 1 ? 1 : 2; // products to a sum
     const auto ranks = [&](int r, auto first) {
-      const auto partsOf = [&](int m, uint32_t (&parts)[PARTS][4]) {
+      const auto partsOf = [&](int step, int m, uint32_t (&parts)[PARTS][4]) {
 #pragma unroll
         for (int part = 0; part < PARTS; part++) {
-          const uint4 q = operands[((m * (c_end / RS) + (r0 + r) / RS) * PARTS + part) * 32];
+          const uint4 q = operands[((m * (c_end / RS) + (r0 + r) / RS + step) * PARTS + part) * 32];
           parts[part][0] = q.x, parts[part][1] = q.y, parts[part][2] = q.z, parts[part][3] = q.w;
         }
       };
-      uint4 b[RS / 4];
-#pragma unroll
-      for (int q = 0; q < RS / 4; q++) {
-        b[q] = r + q * 4 < RC ? shared8B(src + read_b + (r + q * 4) * 64) : make_uint4(0, 0, 0, 0);
-      }
       if constexpr (kPairs<T>) {
-        uint32_t pairs[NJ][2];
-        pairColumns(b, pairs);
+        uint4 b[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          b[q] = r + q * 4 < RC ? shared8B(src + read_b + (r + q * 4) * 64) : make_uint4(0, 0, 0, 0);
+        }
+        uint32_t pairs[1][NJ][2];
+        pairColumns(b, pairs[0]);
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-          uint32_t parts[PARTS][4];
-          partsOf(m, parts);
-          mmaPairs<decltype(first)::value>(acc[m], parts, pairs);
+          uint32_t parts[1][PARTS][4];
+          partsOf(0, m, parts[0]);
+          mmaPairs<decltype(first)::value, 1>(acc[m], parts, pairs);
         }
       } else {
-        mmaColumns<T, decltype(first)::value>(acc, partsOf, b[0], b[1]);
+        uint4 b0[STEPS], b1[STEPS];
+#pragma unroll
+        for (int step = 0; step < STEPS; step++) {
+          b0[step] = shared8B(src + read_b + (r + step * 8) * 64);
+          b1[step] = shared8B(src + read_b + (r + step * 8 + 4) * 64);
+        }
+        mmaColumns<T, decltype(first)::value, STEPS>(acc, partsOf, b0, b1);
       }
     };
     if (NT < 8 || r0 == 0) { // kernels of fewer than 64 ranks have them all in one pass
@@ -897,7 +919,7 @@ __global__ void __launch_bounds__(ApplyShape<MT, NT>::W * 32, (ApplyShape<MT, NT
       ranks(0, std::false_type());
     }
 #pragma unroll
-    for (int r = RS; r < RC; r += RS) {
+    for (int r = RS * STEPS; r < RC; r += RS * STEPS) {
       if (r0 + r < p.rank) {
         ranks(r, std::false_type());
       }
@@ -1024,17 +1046,20 @@ struct Grad {
 constexpr int kGradWarps = 4, kGradRows = 32, kGradStages = 3;
 
 // a stage: 32 rows of 128 bytes for every warp, and the ranks of the same rows of u for all of them (rows of
-// 16 RT + 8 floats: the eight ranks x four rows of a fragment then lie in different banks)
-template <int RT> struct GradShape {
+// 16 RT + 8 floats: the eight ranks x four rows of a fragment then lie in different banks). Behind the ring the parts of
+// u of the present stage, as the products' operands, split once for the four warps (both gradients of 8192 rows 4096 -> 4096
+// rank 32 bf16: 66 us with a split for each warp, 61 with one; 60 with 32 rows to a sum of the matrix unit)
+template <typename T, int RT> struct GradShape {
   static constexpr int US = 16 * RT + 8;
   static constexpr int XB = kGradRows * 128, STAGE = kGradWarps * XB + kGradRows * US * 4;
-  static constexpr int BYTES = kGradStages * STAGE;
+  static constexpr int RING = kGradStages * STAGE, BYTES = RING + kGradRows * 16 * RT * kOperandBytes<T>;
 };
 
 template <typename T, bool VEC, int RT>
 __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradKernel(Grad p) {
-  using Shape = GradShape<RT>;
+  using Shape = GradShape<T, RT>;
   constexpr int E = 16 / sizeof(T), NJ = E, UC = 8 * NJ, S = kGradStages;
+  constexpr int RS = kOperandRanks<T>, PARTS = kPairs<T> ? kParts : 2; // rows to a product
   extern __shared__ __align__(16) unsigned char smem[];
   waitForLaunchBefore();
   const int side = blockIdx.z / p.rank_passes, r0 = (blockIdx.z % p.rank_passes) * 16 * RT;
@@ -1056,6 +1081,7 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
   const int ranks = min(p.rank - r0, 16 * RT);
   const bool u_wide = p.rank % 4 == 0 && (uintptr_t)u % 16 == 0;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem);
+  uint4 *operands = reinterpret_cast<uint4 *>(smem + Shape::RING);
   const int chunks = (tile.rows + kGradRows - 1) / kGradRows;
   const auto fetch = [&](int i, int stage) {
     if (i < chunks) {
@@ -1103,49 +1129,73 @@ __global__ void __launch_bounds__(kGradWarps * 32, RT == 4 ? 2 : 3) lowRankGradK
   }
   for (int i = 0; i < chunks; i++) {
     fetchWait<S - 2>();
-    __syncthreads(); // chunk i is there for all, and all are done with the stage of chunk i - 1
+    __syncthreads(); // chunk i is there for all, and all are done with the stage and the operands of chunk i - 1
     fetch(i + S - 1, (i + S - 1) % S);
     const unsigned char *src = smem + (i % S) * Shape::STAGE;
     const float *us = reinterpret_cast<const float *>(src + kGradWarps * Shape::XB);
     const unsigned char *xs = src + warp * Shape::XB + t * 128 + (g ^ (2 * t)) * 16;
-    const float *uf = us + t * Shape::US + g;
-    if constexpr (kPairs<T>) {
-#pragma unroll 1
-      for (int r = 0; r < kGradRows; r += 16) {
-        uint4 b[4];
+    // the parts of u: [step of RS rows][fragment of 16 ranks][part][lane][4]
+    for (int item = warp; item < kGradRows / RS * RT; item += kGradWarps) {
+      const float *uf = us + (item / RT * RS + t) * Shape::US + item % RT * 16 + g;
+      uint32_t parts[PARTS][4];
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          b[q] = shared16B(xs + (r + 4 * q) * 128);
-        }
-        uint32_t pairs[NJ][2];
-        pairColumns(b, pairs);
+      for (int e = 0; e < 4; e++) {
+        const float *f = uf + (e >> 1) * (RS / 2) * Shape::US + (e & 1) * 8;
+        if constexpr (kPairs<T>) {
+          uint32_t pair[kParts];
+          splitPair(f[0], f[4 * Shape::US], pair);
 #pragma unroll
-        for (int q = 0; q < RT; q++) {
-          uint32_t parts[kParts][4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float *f = uf + (r + (e >> 1) * 8) * Shape::US + q * 16 + (e & 1) * 8;
-            uint32_t pair[kParts];
-            splitPair(f[0], f[4 * Shape::US], pair);
-#pragma unroll
-            for (int part = 0; part < kParts; part++) {
-              parts[part][e] = pair[part];
-            }
+          for (int part = 0; part < kParts; part++) {
+            parts[part][e] = pair[part];
           }
-          mmaPairs<false>(acc[q], parts, pairs);
+        } else {
+          split(f[0], parts[0][e], parts[1][e]);
         }
       }
-    } else {
-#pragma unroll 1
-      for (int r = 0; r < kGradRows; r += 8) {
-        const uint4 x0 = shared16B(xs + r * 128), x1 = shared16B(xs + (r + 4) * 128);
-        const auto partsOf = [&](int q, uint32_t (&parts)[2][4]) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            split(uf[(r + (e >> 1) * 4) * Shape::US + q * 16 + (e & 1) * 8], parts[0][e], parts[1][e]);
+      for (int part = 0; part < PARTS; part++) {
+        operands[(item * PARTS + part) * 32 + lane] = make_uint4(parts[part][0], parts[part][1], parts[part][2], parts[part][3]);
+      }
+    }
+    __syncthreads();
+    constexpr int STEPS = 2; // products to a sum
+#pragma unroll 1
+    for (int r = 0; r < kGradRows; r += RS * STEPS) {
+      const auto partsOf = [&](int step, int q, uint32_t (&parts)[PARTS][4]) {
+#pragma unroll
+        for (int part = 0; part < PARTS; part++) {
+          const uint4 w = operands[(((r / RS + step) * RT + q) * PARTS + part) * 32 + lane];
+          parts[part][0] = w.x, parts[part][1] = w.y, parts[part][2] = w.z, parts[part][3] = w.w;
+        }
+      };
+      if constexpr (kPairs<T>) {
+        uint32_t pairs[STEPS][NJ][2];
+#pragma unroll
+        for (int step = 0; step < STEPS; step++) {
+          uint4 b[4];
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            b[q] = shared16B(xs + (r + step * RS + 4 * q) * 128);
           }
-        };
-        mmaColumns<T, false>(acc, partsOf, x0, x1);
+          pairColumns(b, pairs[step]);
+        }
+#pragma unroll
+        for (int q = 0; q < RT; q++) {
+          uint32_t parts[STEPS][PARTS][4];
+#pragma unroll
+          for (int step = 0; step < STEPS; step++) {
+            partsOf(step, q, parts[step]);
+          }
+          mmaPairs<false, STEPS>(acc[q], parts, pairs);
+        }
+      } else {
+        uint4 x0[STEPS], x1[STEPS];
+#pragma unroll
+        for (int step = 0; step < STEPS; step++) {
+          x0[step] = shared16B(xs + (r + step * RS) * 128);
+          x1[step] = shared16B(xs + (r + step * RS + 4) * 128);
+        }
+        mmaColumns<T, false, STEPS>(acc, partsOf, x0, x1);
       }
     }
   }
@@ -1253,7 +1303,7 @@ template <typename T, bool VEC> void launchGrad(Grad p, long long slots, cudaStr
   const int rt = p.rank <= 16 ? 1 : p.rank <= 32 ? 2 : 4;
   p.rank_passes = (p.rank + 16 * rt - 1) / (16 * rt);
   auto kernel = rt == 1 ? lowRankGradKernel<T, VEC, 1> : rt == 2 ? lowRankGradKernel<T, VEC, 2> : lowRankGradKernel<T, VEC, 4>;
-  const int smem = rt == 1 ? GradShape<1>::BYTES : rt == 2 ? GradShape<2>::BYTES : GradShape<4>::BYTES;
+  const int smem = rt == 1 ? GradShape<T, 1>::BYTES : rt == 2 ? GradShape<T, 2>::BYTES : GradShape<T, 4>::BYTES;
   AB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   // a grid's second dimension takes 65535 blocks: rows of more than 8388480 fp32 columns go in parts
   const int blocks = (widest + uc - 1) / uc;
