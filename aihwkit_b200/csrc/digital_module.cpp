@@ -128,20 +128,22 @@ bool rowDistance(const Tensor &t, int64_t *ld) {
   }
   return true;
 }
+// torch keeps the sign of some views (the imaginary part of a conjugate) apart from their memory
+Tensor signedIn(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 Rows rowsOf(const Tensor &t) {
   Rows r;
   if (!t.defined()) {
     return r;
   }
-  r.t = t;
-  if (!rowDistance(t, &r.ld)) {
-    r.t = t.contiguous();
-    r.ld = t.size(-1);
+  r.t = signedIn(t);
+  if (!rowDistance(r.t, &r.ld)) {
+    r.t = r.t.contiguous();
+    r.ld = r.t.size(-1);
   }
   r.p = r.t.data_ptr();
   return r;
 }
-Tensor whole(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
+Tensor whole(const Tensor &t) { return t.defined() ? signedIn(t).contiguous() : t; }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 void *stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 Tensor optional(const std::optional<Tensor> &t) { return t.has_value() ? *t : Tensor(); }
@@ -493,14 +495,14 @@ Tensor lowRankAdd(const Tensor &base, const Tensor &x, const Tensor &a, const Te
   checkLike(b, "b", x);
   REFUSE(a.dim() != 3 || b.dim() != 3 || a.size(0) != b.size(0) || a.size(1) != b.size(1),
          "a and b must be [adapters, rank, width], got " << a.sizes() << " and " << b.sizes());
-  REFUSE(!a.is_contiguous() || !b.is_contiguous(), "a and b must be contiguous");
+  REFUSE(!a.is_contiguous() || !b.is_contiguous() || a.is_neg() || b.is_neg(), "a and b must be contiguous");
   REFUSE(a.numel() == 0 || b.numel() == 0, "at least one adapter, rank and column is needed");
   REFUSE(x.dim() < 1 || x.size(-1) != a.size(2) || base.dim() < 1 || base.size(-1) != b.size(2),
          "expected x [..., " << a.size(2) << "] and base [..., " << b.size(2) << "], got " << x.sizes() << " and "
                              << base.sizes());
   REFUSE(x.sizes().slice(0, x.dim() - 1) != base.sizes().slice(0, base.dim() - 1), "x and base need the same rows");
   REFUSE(scale.scalar_type() != at::kFloat || scale.device() != x.device() || scale.dim() != 1 ||
-             scale.size(0) != a.size(0) || !scale.is_contiguous(),
+             scale.size(0) != a.size(0) || !scale.is_contiguous() || scale.is_neg(),
          "scale must be a contiguous Float tensor of " << a.size(0) << " values on " << x.device());
   REFUSE(wantsGrad({&scale}), "scale has no gradient here");
   const std::pair<const Tensor *, const char *> tables[] = {{&ids, "adapter_ids"}, {&starts, "row_starts"}};
@@ -525,7 +527,7 @@ Tensor lowRankAdd(const Tensor &base, const Tensor &x, const Tensor &a, const Te
            "out may be base itself, but not a part or another view of it");
     REFUSE(overlap(out, x) || overlap(out, a) || overlap(out, b), "out must not share memory with x, a or b");
     int64_t ld = 0;
-    REFUSE(out.numel() > 0 && (!rowDistance(out, &ld) || (ld < out.size(-1) && rows > 1)),
+    REFUSE(out.numel() > 0 && (out.is_neg() || !rowDistance(out, &ld) || (ld < out.size(-1) && rows > 1)),
            "out must be rows of neighbouring elements with one distance between them");
   } else if (grad) {
     return LowRankAdd::apply(base, x, a, b, scale, ids, given(starts));
