@@ -522,7 +522,8 @@ Tensor lowRankAdd(const Tensor &base, const Tensor &x, const Tensor &a, const Te
   const bool grad = wantsGrad({&base, &x, &a, &b});
   if (out.defined()) {
     checkSame(out, "out", base);
-    REFUSE(grad, "out= is for calls without gradients");
+    // an `out` with a history of its own would keep it, and pass the result's gradient on to what it was before
+    REFUSE(grad || wantsGrad({&out}), "out= is for calls without gradients");
     REFUSE((out.strides() != base.strides() || out.data_ptr() != base.data_ptr()) && overlap(out, base),
            "out may be base itself, but not a part or another view of it");
     REFUSE(overlap(out, x) || overlap(out, a) || overlap(out, b), "out must not share memory with x, a or b");
