@@ -6,7 +6,7 @@
 //
 // lowRankApplyKernel. The work is narrow: 2 rank operations per element of x and of y, so memory
 // bounds it up to ranks of about 64. A block takes up to 64 (32, 16) rows of one request through both
-// products: x is read once, v stays in shared memory, y is written once; nothing but the saved v
+// products: x is read once (above 64 ranks once for every 64), v stays in shared memory, y is written once; nothing but the saved v
 // goes through memory between the two. A dot product may run in any order, so a thread takes 16
 // neighbouring bytes of a row as its share of k, and columns are dealt to the fragments of mma.sync so that it ends up
 // with 16 neighbouring bytes of y. Every warp has its own steps along k and its own columns and
@@ -19,15 +19,16 @@
 // 2^-22 of a product out. Where v (or u of the gradients) meets bf16, its three parts are bf16 and hold all of its 24
 // bits, three products in place of the four that TF32 parts take at half the rate. fp16 has not the range for that.
 //
-// Measured: 16384 rows 768 -> 2304 rank 16 in 16 requests, fp32 70 us (5.0 TB/s), bf16 37 us (4.8 TB/s); 8192 rows 4096 ->
-// 4096 bf16, rank 32 47 us (4.3 TB/s), rank 64 71 us; 256 tokens of 64 adapters 4096 -> 4096 rank 16 15 us. 16 warps or fewer
-// fit a multiprocessor (registers, rings), and what they wait for - loads, shared memory, their own products - bounds
-// it; no pipe is more than 45 % busy.
+// Measured: 16384 rows 768 -> 2304 rank 16 in 16 requests, fp32 70 us (5.0 TB/s), bf16 38 us (4.6 TB/s); 8192 rows 4096 ->
+// 4096 bf16, rank 32 52 us (3.9 TB/s), rank 64 84 us, rank 128 151 us (rank 32 and 64 took 47 and 71 us with v in two bf16 parts);
+// 256 tokens of 64 adapters 4096 -> 4096 rank 16 15 us. 16 warps or fewer fit a multiprocessor (registers, rings), and what
+// they wait for - loads, shared memory, their own products - bounds it; issue slots are up to 45 % busy, no pipe more than 36 %.
 //
 // lowRankGradKernel. grad[id] = sum over the rows of id of u^T x: a warp holds rank x 128 bytes of columns
 // in fragments and walks a chunk of rows of one request, fetched the same way; chunks' partial sums go
 // through memory and are added in the order of the rows (no atomics). Measured: both gradients of 8192 rows 4096 -> 4096
-// rank 32 bf16 39 us (3.4 TB/s of x and gy), 61 us while the partial sums were stored by single floats.
+// rank 32 bf16 54 us and 10 us for the chunks' sums (39 and 8 with u in two bf16 parts and one sum of the matrix unit over
+// all rows), with 10 warps to a multiprocessor and the matrix pipe half busy.
 #include "digital.cuh"
 
 #include <algorithm>

@@ -7,8 +7,11 @@ are torch calls around ``AnalogLinear``; here they are kernels of the library (`
 
 All of them take CUDA tensors of float32, float16 or bfloat16 whose last dimension lies together in memory (others are
 copied first), run on the current stream of the tensors' device, wait for nothing and raise ``RuntimeError`` for what they
-do not take.  Sums, means and products are held in fp32; results are rounded once.  They can be captured into a CUDA
-graph; a captured dropout repeats the ``call`` it was captured with.
+do not take.  Sums and means are held in fp32 and results are rounded once.  In the products of the adapters 16-bit factors are
+exact; fp32 ones (all of an fp32 call, and ``x a^T`` or ``gy b^T`` on the way into the second product) have at least 22 of their
+24 bits there, beside bfloat16 all.  Gradients are those of reverse mode, once: second derivatives, forward mode, tracing and
+``torch.func`` are refused.  The calls can be captured into a CUDA graph; a captured dropout repeats the ``call`` it was
+captured with.
 """
 
 from __future__ import annotations

@@ -795,8 +795,10 @@ int ab200_mvm_forward_noalloc(const ab200_io_params *forward_io, const float *w_
  * (a stride of 0 repeats one row and is for inputs only). Infinities and NaN make the results not finite that
  * are summed from them, and no others. Nothing is allocated and nothing is waited
  * for; the calls can be captured into a graph. Sums, means and saved values are fp32 whatever the type,
- * results are rounded once. Outputs must not overlap inputs unless a call says so. Pointers lie on multiples of
- * their elements' size, the workspace of ab200_low_rank_grad on one of 16 bytes. */
+ * results are rounded once. In the products of the low-rank adapters 16-bit factors are exact; fp32 ones (all
+ * of fp32 calls, v and u) have at least 22 of their 24 bits there, beside bf16 all. Outputs must not overlap
+ * inputs unless a call says so. Pointers lie on multiples of their elements' size, the workspace of
+ * ab200_low_rank_grad on one of 16 bytes. */
 enum ab200_dtype { AB200_DTYPE_F32 = 0, AB200_DTYPE_F16 = 1, AB200_DTYPE_BF16 = 2 };
 
 /* y = keep ? x / (1 - p) : 0, plus `residual` where it is not null. A dropped element is 0 whatever it
@@ -844,8 +846,9 @@ int ab200_layer_norm_backward(const void *gy, long long gy_stride, const void *g
  * The gradient of x is the same call on gy with a and b (k and n) exchanged, its v what the
  * gradient of a needs (u below).
  * grad: da = sum over an adapter's rows of u^T x, db = sum of v^T gy, of the type of x and gy, zero for
- * adapters without rows; each may be null. The workspace has rank * (k + n) floats for every request at least. workspace has the bytes that ab200_low_rank_grad_workspace
- * gives for the same sizes (k or n 0 where that gradient is not wanted; one_row_each: row_starts is null).
+ * adapters without rows; each may be null. workspace has the bytes that ab200_low_rank_grad_workspace gives for the same
+ * sizes (k or n 0 where that gradient is not wanted; one_row_each: row_starts is null), rank * (k + n) floats for every
+ * request at least.
  * Requests may share an adapter; sums over rows are added in the order of the rows. Rows of one adapter
  * cost least as one request: each request has tiles of its own. */
 int ab200_low_rank_apply(const void *x, long long x_stride, const void *base, long long base_stride,
